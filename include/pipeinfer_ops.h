@@ -477,6 +477,35 @@ PI_API int pi_op_diff_attention(const float * q_dev, int64_t q_stride, const flo
                                 int keep_first, int maps, float lam, float out_mult, float eps, int heads, int kv_heads, int dim, int vdim, int n_tok, int n_kv, float * scratch_dev, size_t scratch_floats, float * out_dev,
                                 int64_t out_stride, const int32_t * dyn_dev, void * stream);
 
+/* ---- operators of a batch of continuations of one prompt: attention over cells that all of them see, what every cell was given, a cut of the cache, a token for every row -------- */
+/* Soft-max attention over the caches of pi_op_attention (fp16 rows of n_head_kv * head_dim values per cell), all in fp32 between the products, whose tokens share their first cells:
+ *   s = q . k * scale;  lse[t][h] = log sum exp(s);  out[t][h] = sum exp(s - lse) v       over the cells [0, n_prompt), which every token sees, and the cells [n_prompt, n_kv) whose bit of the token's mask is set
+ * Keys and values of the prompt are read once for all tokens; a cell behind it is read for the tokens that see it, and what stands in the others is without effect (as are the mask's bits below n_prompt).  A token that sees nothing: zeros
+ * and minus infinity.  q16: rows q_stride halves apart (a multiple of 8); out: rows out_stride floats apart (a multiple of 4); lse: fp32 [n_tok][n_head], nullable; mask as for pi_op_attention, nullable without such cells; heads of
+ * 8 .. 256 values in steps of 8; scale positive; q16, caches, out and scratch on 16 bytes.
+ * dyn_dev (nullable): int32 {n_prompt, n_kv} in device memory, at most the arguments, which then size the split of the work and the mask's rows.  One scratch (pi_op_prefix_attention_scratch_floats; 0: none) per pass in flight */
+PI_API int pi_op_prefix_attention(const uint16_t * q16_dev, int64_t q_stride, const uint16_t * k_cache_dev, const uint16_t * v_cache_dev, const uint32_t * mask_dev, float scale, int head_dim, int n_head, int n_head_kv, int n_tok,
+                                  int n_prompt, int n_kv, float * scratch_dev, size_t scratch_floats, float * out_dev, int64_t out_stride, float * lse_dev, const int32_t * dyn_dev, void * stream);
+PI_API size_t pi_op_prefix_attention_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv);
+/* What the soft-maxes of such a pass gave every cell: mass[c] <- decay * mass[c] + sum over the tokens and heads that see cell c of exp(s - lse[t][h])   (decay 0: the old mass is not read).  lse as pi_op_prefix_attention leaves it
+ * (minus infinity: the row gives nothing); cells, mask, scratch and dyn_dev as there.  mass: fp32 [n_kv].  Without tokens nothing happens */
+PI_API int pi_op_attention_mass(const uint16_t * q16_dev, int64_t q_stride, const uint16_t * k_cache_dev, const uint32_t * mask_dev, const float * lse_dev, float scale, int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt,
+                                int n_kv, float decay, float * scratch_dev, size_t scratch_floats, float * mass_dev, const int32_t * dyn_dev, void * stream);
+PI_API size_t pi_op_attention_mass_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv);
+/* Which cells stay when a cache of `cells` is cut to `keep`: the guarded ones (bitmap, nullable; the lower indices where they are more), then those of the largest mass; the lower index wins a tie, what is no number comes last.  source [keep]: the cell whose rows belong
+ * at i: i itself for a cell in front that stays; the other places take the cells from behind `keep` that stay, both in ascending order */
+PI_API int pi_op_cache_choose(const float * mass_dev, const uint32_t * guard_dev, int cells, int keep, int32_t * source_dev, void * stream);
+/* row i <- row source[i] of n_arrays arrays (their device addresses and rows' bytes in host memory) for every i < keep with keep <= source[i] < cells; other entries move nothing */
+PI_API int pi_op_cache_move(void * const * arrays_dev, const int64_t * row_bytes, int n_arrays, const int32_t * source_dev, int keep, int cells, void * stream);
+/* A token for every row of logits (rows `stride` floats apart, at most 524288 logits) from a given random number, settings per row (each nullable: off):
+ *   the first top_k (<= 0: all) in the order of falling logits (lower id on a tie); of those, with w = exp(x - max), the ones whose weights ahead of them sum to less than top_p * (all weights) (>= 1: all); of those the ones with
+ *   w >= min_p; the first always stays.  e = exp((x - max) / temp) of what stays (temp <= 0: the first alone); id: the first, by id, whose running sum of e exceeds u * (the sum of e), u in [0, 1)
+ * prob (nullable): e / sum of the token; kept (nullable): how many stayed.  Minus infinity and NaN are not there; a row of nothing else gives id -1, prob 0, kept 0.  Sums are held in steps of 2^-44 of the largest weight (smaller ones are
+ * not drawn), so that the same inputs give the same token whatever runs beside */
+PI_API int pi_op_sample(const float * logits_dev, int64_t stride, int n_vocab, int rows, const float * temp_dev, const int32_t * top_k_dev, const float * top_p_dev, const float * min_p_dev, const float * u_dev, void * scratch_dev,
+                        size_t scratch_bytes, int32_t * id_dev, float * prob_dev, int32_t * kept_dev, void * stream);
+PI_API size_t pi_op_sample_scratch_bytes(int n_vocab, int rows);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,588 @@
+// Attention of a batch whose tokens share their first cells, and what every cell has been given by it.
+//
+//   s = q . k * scale,  p = exp(s - lse),  lse = log sum exp(s),  out = sum p v          over the cells [0, prompt) for every token, and behind them over the cells whose mask bit is set
+//   mass[cell] <- decay * mass[cell] + sum over the tokens and heads that see it of p
+//
+// The query rows of a key head - tokens x its query heads - are one matrix against the prompt's keys, so a key is read once for all of them.  The cells behind the prompt differ from token to token: a workgroup takes one
+// token's, listed from its mask, and reads no other, so that what stands in the others is without effect.  Scores are computed transposed (rows = cells): what a lane then holds - sixteen cells of one query - is, eight at a time, the
+// operand of the product with the values, and the values come from LDS through its transposing load.
+// Sums and statistics are fp32.  Products are fp16 x fp16 (exact in fp32); a weight is two fp16 values, what the first leaves and the second again cuts off (22 bits; one alone, 11 bits, is 1.4e-4 off over 32000 cells).
+#include "ops_common.h"
+#include "kernel_timing.h"
+
+#include <algorithm>
+#include <cmath>
+
+typedef _Float16 px_half8 __attribute__((ext_vector_type(8)));
+typedef __fp16 px_half2 __attribute__((ext_vector_type(2)));
+typedef short px_short4 __attribute__((ext_vector_type(4)));
+typedef uint32_t px_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t px_u32x2 __attribute__((ext_vector_type(2)));
+typedef float px_f32x16 __attribute__((ext_vector_type(16)));
+typedef float px_f32x4 __attribute__((ext_vector_type(4)));
+
+static __device__ __forceinline__ px_f32x16 px_mfma(px_u32x4 a, px_u32x4 b, px_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(px_half8, a), __builtin_bit_cast(px_half8, b), c, 0, 0, 0); }
+static __device__ __forceinline__ px_f32x16 px_zero() { return px_f32x16{ 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f }; }
+// the cell of register i of a tile's scores, lane half g
+static __device__ __forceinline__ int px_cell(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
+
+// Bytes between rows in LDS.  Keys: an odd number of 16 bytes, so that the rows of a read of 16 bytes a lane lie apart.  Values: a transposing read takes 64 bytes of four rows for 32 lanes: 64 or 192 modulo 256
+template <int DP> struct px_lds { static constexpr int K = 2 * DP + 16, V = (DP / 32) % 2 ? 2 * DP : 2 * DP + 64; };
+
+#define PX_LIFT 6.0f        /* weights are held times 2^6, 2^14 where the maximum lags: fp16's smallest steps are then 2^-30 of the largest weight */
+#define PX_LAG 8.0f         /* the maximum that weights are relative to follows when it has grown by 2^8 */
+#define PX_LIST 8192        /* cells of 256 words of a mask */
+
+// 32 queries of one key head, a column of the tile per lane, lanes l and l + 32 the same: their sums so far.  Of acc the outputs 32 j + px_cell(i, g); m in powers of two, l of the lane's own cells
+template <int DP> struct px_sums { px_f32x16 acc[DP / 32]; float m, l; };
+template <int DP> static __device__ __forceinline__ void px_start(px_sums<DP> & S) {
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++) S.acc[j] = px_zero();
+    S.m = -INFINITY; S.l = 0.0f;
+}
+
+// a tile of 32 cells, of which the first `live` count: key(i) gives the operand of its values 16 i + 8 g .., value(j, z) that of the outputs 32 j .. and the cells 16 z ..; c = scale * log2(e)
+template <int DP, class K, class V> static __device__ __forceinline__ void px_tile(px_sums<DP> & S, const px_u32x4 (&q)[DP / 16], float c, int live, int g, K && key, V && value) {
+    px_f32x16 s = px_zero();
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) s = px_mfma(key(i), q[i], s);
+    if (live < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) if (px_cell(i, g) >= live) s[i] = -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+    top = fmaxf(top, s[15]);
+    top = fmaxf(top, pi_partner<32>(top)) * c;
+    if (__any(top > S.m + PX_LAG)) {
+        const float m = fmaxf(S.m, top), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);
+        S.m = m; S.l *= f;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) S.acc[j][i] *= f;
+    }
+    const float lift = PX_LIFT - (S.m == -INFINITY ? 0.0f : S.m);
+    float p[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, lift));
+    S.l += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) + (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+    px_u32x4 hi[2], lo[2];
+#pragma unroll
+    for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = p[8 * z + 2 * e], b = p[8 * z + 2 * e + 1];
+            const px_half2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
+            hi[z][e] = __builtin_bit_cast(uint32_t, h);
+            lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], -1.0f, a), fmaf((float) h[1], -1.0f, b)));
+        }
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            const px_u32x4 v = value(j, z);
+            S.acc[j] = px_mfma(v, hi[z], S.acc[j]);
+            S.acc[j] = px_mfma(v, lo[z], S.acc[j]);
+        }
+}
+
+// the values' operand from rows of `stride` bytes in LDS: at = the wave's first row + px_value_at; sixteen lanes take four rows of sixteen values and each gets a column
+static __device__ __forceinline__ int px_value_at(int lane, int stride) { return ((lane & 15) / 4 + 4 * (lane >> 5)) * stride + 32 * (lane >> 4 & 1) + 8 * (lane & 3); }
+template <int STRIDE> static __device__ __forceinline__ px_u32x4 px_value(const uint8_t * at, int j, int z) {
+    typedef __attribute__((address_space(3))) px_short4 lds4;
+    const px_u32x2 a = __builtin_bit_cast(px_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 16 * z * STRIDE + 64 * j)));
+    const px_u32x2 b = __builtin_bit_cast(px_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + (16 * z + 8) * STRIDE + 64 * j)));
+    return px_u32x4{ a[0], a[1], b[0], b[1] };
+}
+
+struct px_args {
+    const uint16_t * q; int64_t q_stride;
+    const uint16_t * k, * v; int64_t row;                    // a cell's values: all key heads
+    const uint32_t * mask; const int32_t * dyn;
+    float c;
+    int dim, heads, kv, group, n_tok, prompt, n_kv;
+    int rows_of, row_blocks, prompt_parts, own_blocks, own_parts;   // rows of a workgroup; of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
+    float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
+    float * out; int64_t out_stride; float * lse;
+};
+
+// the sums of 32 rows of key head j from row0 on: part `part` of theirs, or the result where it is the only one
+template <int DP> static __device__ __forceinline__ void px_leave(const px_args & A, px_sums<DP> & S, int part, int tok, int head, bool mine, int g) {
+    const float l = S.l + pi_partner<32>(S.l);
+    if (!mine) return;
+    const bool last = A.prompt_parts + A.own_parts == 1;
+    const int64_t r = (int64_t) tok * A.heads + head;
+    float * o;
+    float f = 1.0f;
+    if (last) {
+        o = A.out + (int64_t) tok * A.out_stride + (int64_t) head * A.dim;
+        f = l == 0.0f ? 0.0f : 1.0f / l;
+        if (g == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (S.m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+    } else {
+        const int64_t at = (int64_t) part * A.n_tok * A.heads + r;
+        o = A.parts_o + at * A.dim;
+        if (g == 0) A.parts_ml[at] = make_float2(S.m, l);
+        if (l == 0.0f) return;                               // (k_prefix_merge leaves such a part out)
+    }
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * j + px_cell(i, g);
+            if (d < A.dim) *(px_f32x4 *) (o + d) = px_f32x4{ S.acc[j][i] * f, S.acc[j][i + 1] * f, S.acc[j][i + 2] * f, S.acc[j][i + 3] * f };
+        }
+}
+
+template <int DP> static __device__ __forceinline__ void px_queries(const px_args & A, px_u32x4 (&q)[DP / 16], int tok, int head, int g) {
+    const uint16_t * row = A.q + (int64_t) tok * A.q_stride + (int64_t) head * A.dim;
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) q[i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (row + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+}
+
+// Many rows: a wave has 32 of the workgroup's 128, all walk the same cells.  Tiles of 64 cells, two in LDS: while one is worked on the next is on its way in registers
+template <int DP> static __device__ __forceinline__ void px_wide(const px_args & A, uint8_t * lds, int kvh, int block, int part, int c0, int c1) {
+    constexpr int KS = px_lds<DP>::K, VS = px_lds<DP>::V, STAGE = 64 * (KS + VS), N = DP / 32, CH = DP / 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5, rows = A.n_tok * A.group;
+    const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = at / A.group, head = kvh * A.group + at % A.group;
+    px_u32x4 q[DP / 16], kr[N], vr[N];
+    px_queries<DP>(A, q, tok, head, g);
+    px_sums<DP> S;
+    px_start(S);
+    const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
+    auto load = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int x = i * 256 + tid, d = x % CH * 8;
+            const int64_t o = (int64_t) min(c + x / CH, c1 - 1) * A.row + d;
+            kr[i] = d < A.dim ? *(const px_u32x4 *) (k + o) : px_u32x4{ 0, 0, 0, 0 };
+            vr[i] = d < A.dim ? *(const px_u32x4 *) (v + o) : px_u32x4{ 0, 0, 0, 0 };
+        }
+    };
+    auto store = [&](uint8_t * to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int x = i * 256 + tid;
+            *(px_u32x4 *) (to + x / CH * KS + x % CH * 16) = kr[i];
+            *(px_u32x4 *) (to + 64 * KS + x / CH * VS + x % CH * 16) = vr[i];
+        }
+    };
+    load(c0);
+    store(lds);
+    int cur = 0;
+    for (int c = c0; c < c1; c += 64, cur ^= 1) {
+        __syncthreads();
+        const bool more = c + 64 < c1;
+        if (more) load(c + 64);
+        const uint8_t * st = lds + cur * STAGE;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (c + 32 * u >= c1) continue;
+            const uint8_t * kt = st + (32 * u + n) * KS + 16 * g, * vt = st + 64 * KS + 32 * u * VS + px_value_at(lane, VS);
+            px_tile<DP>(S, q, A.c, c1 - c - 32 * u, g, [&](int i) __attribute__((always_inline)) { return *(const px_u32x4 *) (kt + 32 * i); },
+                        [&](int j, int z) __attribute__((always_inline)) { return px_value<VS>(vt, j, z); });
+        }
+        if (more) store(lds + (cur ^ 1) * STAGE);
+    }
+    px_leave<DP>(A, S, part, tok, head, row < rows, g);
+}
+
+// Few rows, 32 of them to a workgroup: its waves walk every fourth run of 32 cells each and meet at the end.  `count` cells, the i-th of them at cell_of(i); sums go on in S.  Keys come as operands, values to a part of LDS that is the wave's
+// own, so that no wave waits for another; the next run's are on their way meanwhile
+template <int DP, class C> static __device__ __forceinline__ void px_walk(const px_args & A, px_sums<DP> & S, const px_u32x4 (&q)[DP / 16], uint8_t * mine, int kvh, int wave, int lane, int count, C && cell_of) {
+    constexpr int VS = px_lds<DP>::V, CH = DP / 8, N = DP / 16;
+    const int n = lane & 31, g = lane >> 5;
+    const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
+    px_u32x4 kr[N], vr[N];
+    auto load = [&](int at) __attribute__((always_inline)) {
+        const int64_t o = (int64_t) cell_of(min(at + n, count - 1)) * A.row;
+#pragma unroll
+        for (int i = 0; i < N; i++) kr[i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (k + o + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int x = i * 64 + lane, d = x % CH * 8;
+            vr[i] = d < A.dim ? *(const px_u32x4 *) (v + (int64_t) cell_of(min(at + x / CH, count - 1)) * A.row + d) : px_u32x4{ 0, 0, 0, 0 };
+        }
+    };
+    if (32 * wave >= count) return;
+    load(32 * wave);
+    for (int at = 32 * wave; at < count; at += 128) {
+        px_u32x4 kc[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            kc[i] = kr[i];
+            const int x = i * 64 + lane;
+            *(px_u32x4 *) (mine + x / CH * VS + x % CH * 16) = vr[i];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        if (at + 128 < count) load(at + 128);
+        const uint8_t * vt = mine + px_value_at(lane, VS);
+        px_tile<DP>(S, q, A.c, count - at, g, [&](int i) __attribute__((always_inline)) { return kc[i]; }, [&](int j, int z) __attribute__((always_inline)) { return px_value<VS>(vt, j, z); });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// the sums of the four waves into the first one's, two at a time; lds: 2 * (DP + 2) * 256 bytes, no wave in its own part any more
+template <int DP> static __device__ __forceinline__ void px_meet(px_sums<DP> & S, uint8_t * lds, int wave, int lane) {
+    S.l += pi_partner<32>(S.l);
+    float * at = (float *) lds + (wave & 1) * (DP / 2 + 2) * 64 + lane;
+#pragma unroll
+    for (int half = 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            float * to = (float *) lds + (wave - half) * (DP / 2 + 2) * 64 + lane;
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) to[(16 * j + i) * 64] = S.acc[j][i];
+            to[DP / 2 * 64] = S.m; to[(DP / 2 + 1) * 64] = S.l;
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float om = at[DP / 2 * 64], ol = at[(DP / 2 + 1) * 64], m = fmaxf(S.m, om);
+            const float a = S.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(S.m - m), b = om == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(om - m);
+            S.m = m; S.l = S.l * a + ol * b;
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) S.acc[j][i] = S.acc[j][i] * a + at[(16 * j + i) * 64] * b;
+        }
+    }
+    S.l *= 0.5f;                                             // (px_leave adds the halves)
+}
+
+// part `part` of `parts` of n things in runs of `run`
+static __device__ __forceinline__ void px_share(int n, int run, int part, int parts, int & from, int & to) {
+    const int64_t runs = (n + run - 1) / run;
+    from = (int) min((int64_t) n, runs * part / parts * run); to = (int) min((int64_t) n, runs * (part + 1) / parts * run);
+}
+
+template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
+    if (pi_aborted(abort_w, 5)) return;
+    constexpr int NARROW = 4 * 32 * px_lds<DP>::V + 2 * PX_LIST, MEET = 2 * (DP / 2 + 2) * 256, WIDE_B = WIDE ? 2 * 64 * (px_lds<DP>::K + px_lds<DP>::V) : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? (NARROW > MEET ? NARROW : MEET) : WIDE_B];
+    __shared__ int listed[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
+    const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv);
+    const int pairs = A.kv * A.prompt_parts, prompt_blocks = pairs * A.row_blocks;
+    px_u32x4 q[DP / 16];
+    px_sums<DP> S;
+    uint8_t * mine = lds + wave * 32 * px_lds<DP>::V;
+    if ((int) blockIdx.x < prompt_blocks) {
+        // the blocks of rows that read the same keys follow each other on one XCD (a workgroup's is its number modulo 8)
+        int b = blockIdx.x, pair = b / A.row_blocks, block = b % A.row_blocks;
+        if (pairs % 8 == 0) { pair = b / (8 * A.row_blocks) * 8 + b % 8; block = b / 8 % A.row_blocks; }
+        const int kvh = pair % A.kv, part = pair / A.kv;
+        int c0, c1;
+        px_share(prompt, WIDE ? 64 : 32, part, A.prompt_parts, c0, c1);
+        if constexpr (WIDE) {
+            if (c0 >= c1) {                                  // (fewer cells than there may be)
+                px_start(S);
+                const int row = block * 128 + wave * 32 + n, rows = A.n_tok * A.group, at = min(row, rows - 1);
+                px_leave<DP>(A, S, part, at / A.group, kvh * A.group + at % A.group, row < rows, g);
+            } else px_wide<DP>(A, lds, kvh, block, part, c0, c1);
+        } else {
+            const int rows = A.n_tok * A.group, row = block * 32 + n, at = min(row, rows - 1), tok = at / A.group, head = kvh * A.group + at % A.group;
+            px_queries<DP>(A, q, tok, head, g);
+            px_start(S);
+            px_walk<DP>(A, S, q, mine, kvh, wave, lane, c1 - c0, [&](int i) __attribute__((always_inline)) { return c0 + i; });
+            px_meet<DP>(S, lds, wave, lane);
+            if (wave == 0) px_leave<DP>(A, S, part, tok, head, row < rows, g);
+        }
+        return;
+    }
+    // a token's own cells: 32 of the query heads of one key head
+    int b = blockIdx.x - prompt_blocks;
+    const int kvh = b % A.kv, block = b / A.kv % A.own_blocks, part = b / (A.kv * A.own_blocks) % A.own_parts, tok = b / (A.kv * A.own_blocks * A.own_parts);
+    const int in = block * 32 + n, head = kvh * A.group + min(in, A.group - 1), words = (A.n_kv + 31) / 32, w0 = prompt / 32, w_all = (n_kv + 31) / 32 - w0;
+    uint16_t * list = (uint16_t *) (lds + 4 * 32 * px_lds<DP>::V);
+    px_queries<DP>(A, q, tok, head, g);
+    px_start(S);
+    int from, to;
+    px_share(max(0, w_all), 8, part, A.own_parts, from, to);
+    for (int w = from; w < to; w += 256) {
+        uint32_t bits = 0;
+        if (w + tid < to) {
+            const int at = w0 + w + tid;
+            bits = A.mask[(int64_t) tok * words + at];
+            if (32 * at < prompt) bits &= ~0u << (prompt - 32 * at);            // (prompt - 32 * at < 32: at >= prompt / 32)
+            if (n_kv - 32 * at < 32) bits &= (1u << (n_kv - 32 * at)) - 1;
+        }
+        int before = __popc(bits);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(before, o, 64); if (lane >= o) before += x; }
+        __syncthreads();                                     // (the last round's list has been read)
+        if (lane == 63) listed[wave] = before;
+        __syncthreads();
+        int count = 0;
+        for (int i = 0; i < 4; i++) { if (i < wave) before += listed[i]; count += listed[i]; }
+        before -= __popc(bits);
+        for (uint32_t left = bits; left; left &= left - 1) list[before++] = (uint16_t) (32 * tid + __builtin_ctz(left));
+        __syncthreads();
+        const int first = 32 * (w0 + w);
+        px_walk<DP>(A, S, q, mine, kvh, wave, lane, count, [&](int i) __attribute__((always_inline)) { return first + list[i]; });
+    }
+    px_meet<DP>(S, lds, wave, lane);
+    if (wave == 0) px_leave<DP>(A, S, A.prompt_parts + part, tok, head, in < A.group, g);
+}
+
+// a wave per row: the parts' sums over their joint maximum
+__global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, const int32_t * __restrict__ abort_w) {
+    if (pi_aborted(abort_w, 5)) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = (int64_t) A.n_tok * A.heads, r = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    float m = -INFINITY, l = 0.0f, o[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+    for (int p = lane; p < parts; p += 64) { const float2 x = A.parts_ml[p * rows + r]; if (x.y != 0.0f) m = fmaxf(m, x.x); }
+    m = pi_wave_max(m);
+    for (int p = 0; p < parts; p++) {
+        const float2 x = A.parts_ml[p * rows + r];
+        if (x.y == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f(x.x - m);
+        l += x.y * f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) { const int d = 64 * i + lane; if (d < A.dim) o[i] += A.parts_o[(p * rows + r) * A.dim + d] * f; }
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    float * to = A.out + r / A.heads * A.out_stride + r % A.heads * A.dim;
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const int d = 64 * i + lane; if (d < A.dim) to[d] = o[i] * f; }
+    if (lane == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+}
+
+// ---- how the work is cut ---------------------------------------------------------------------------------------------------------------------------------------------------------------
+static bool px_wide_rows(int rows) { return rows > 64; }
+static void px_plan(px_args & A) {
+    const int rows = A.n_tok * A.group, target = 2 * pi_cu_count();
+    const bool wide = px_wide_rows(rows);
+    A.row_blocks = wide ? (rows + 127) / 128 : (rows + 31) / 32;
+    A.own_blocks = (A.group + 31) / 32;
+    const int64_t units = (int64_t) A.kv * A.row_blocks, own = (int64_t) A.n_tok * A.kv * A.own_blocks;
+    const int span = A.n_kv - A.prompt / 32 * 32;
+    A.prompt_parts = A.prompt == 0 ? 0 : (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256));
+    A.own_parts = A.n_kv == A.prompt ? 0 : (int) std::max<int64_t>(1, std::min<int64_t>(target / own, (span + 511) / 512));
+}
+
+static int px_sizes(const char * what, int dim, int heads, int kv, int n_tok, int prompt, int n_kv) {
+    if (heads < 1 || kv < 1 || heads % kv || dim < 8 || dim > 256 || dim % 8) { pi_set_error("%s: %d query heads over %d key / value heads of %d values (whole groups; 8 .. 256 values in steps of 8)", what, heads, kv, dim); return -1; }
+    if (n_tok < 0 || prompt < 0 || prompt > n_kv || n_kv > 0x7fffff00 || (int64_t) n_tok * heads > 0x3fffffff) { pi_set_error("%s: %d tokens of %d heads, %d of %d cells shared", what, n_tok, heads, prompt, n_kv); return -1; }
+    return 0;
+}
+
+static size_t px_floats(const px_args & A) {
+    const size_t parts = (size_t) A.prompt_parts + A.own_parts;
+    return parts > 1 ? parts * A.n_tok * A.heads * (A.dim + 2) : 0;
+}
+
+extern "C" size_t pi_op_prefix_attention_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv) {
+    if (px_sizes("pi_op_prefix_attention_scratch_floats", head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0 || n_tok == 0) return 0;
+    px_args A{};
+    A.dim = head_dim; A.heads = n_head; A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.prompt = n_prompt; A.n_kv = n_kv;
+    px_plan(A);
+    return px_floats(A);
+}
+
+template <int DP> static int px_launch(const px_args & A, hipStream_t s) {
+    const int64_t blocks = (int64_t) A.kv * A.prompt_parts * A.row_blocks + (int64_t) A.n_tok * A.kv * A.own_blocks * A.own_parts;
+    if (blocks > 0x7fffffff) { pi_set_error("pi_op_prefix_attention: %lld workgroups", (long long) blocks); return -1; }
+    const int parts = A.prompt_parts + A.own_parts, nta = std::min(A.n_tok, PI_KT_MAXNT - 1), acct = pi_account_n_kv() > 0 ? pi_account_n_kv() : A.n_kv;
+    const double bytes = 4.0 * acct * A.row + 6.0 * A.n_tok * A.heads * A.dim;
+    if (blocks > 0) {
+        if (px_wide_rows(A.n_tok * A.group)) PI_KT_LAUNCH(PI_KT_ATT, 0, nta, bytes, (k_prefix_attention<DP, true>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
+        else PI_KT_LAUNCH(PI_KT_ATT, 0, nta, bytes, (k_prefix_attention<DP, false>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
+        PI_CHECK_LAUNCH();
+    }
+    if (parts != 1) {
+        const unsigned grid = (unsigned) (((int64_t) A.n_tok * A.heads + 3) / 4);
+        PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 4.0 * A.n_tok * A.heads * ((double) parts * (A.dim + 2) + A.dim), k_prefix_merge, dim3(grid), dim3(256), 0, s, A, parts, pi_abort_word());
+        PI_CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+#define PX_BY_DIM(GO) (A.dim <= 32 ? GO(32) : A.dim <= 64 ? GO(64) : A.dim <= 96 ? GO(96) : A.dim <= 128 ? GO(128) : A.dim <= 192 ? GO(192) : GO(256))
+
+extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, const uint16_t * k_cache, const uint16_t * v_cache, const uint32_t * mask, float scale, int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt,
+                                      int n_kv, float * scratch, size_t scratch_floats, float * out, int64_t out_stride, float * lse, const int32_t * dyn, void * stream) {
+    const char * what = "pi_op_prefix_attention";
+    if (px_sizes(what, head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0) return -1;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) { pi_set_error("%s: scale %g (positive)", what, (double) scale); return -1; }
+    if (n_tok == 0) return 0;
+    if (!q16 || !out || (n_kv > 0 && (!k_cache || !v_cache)) || (!mask && n_kv > n_prompt)) { pi_set_error("%s: queries, caches, output or mask are NULL", what); return -1; }
+    if (q_stride < (int64_t) n_head * head_dim || q_stride % 8 || out_stride < (int64_t) n_head * head_dim || out_stride % 4 || (((uintptr_t) q16 | (uintptr_t) k_cache | (uintptr_t) v_cache | (uintptr_t) out) & 15)) {
+        pi_set_error("%s: rows of queries and outputs hold %d heads, %lld / %lld values apart (multiples of 8 / 4), all on 16 bytes", what, n_head, (long long) q_stride, (long long) out_stride);
+        return -1;
+    }
+    px_args A{};
+    A.q = q16; A.q_stride = q_stride; A.k = k_cache; A.v = v_cache; A.row = (int64_t) n_head_kv * head_dim; A.mask = mask; A.dyn = dyn; A.c = scale * 1.44269504f;
+    A.dim = head_dim; A.heads = n_head; A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.prompt = n_prompt; A.n_kv = n_kv; A.out = out; A.out_stride = out_stride; A.lse = lse;
+    px_plan(A);
+    const size_t need = px_floats(A);
+    if (need > 0 && (!scratch || ((uintptr_t) scratch & 15) || scratch_floats < need)) { pi_set_error("%s: %zu floats of scratch, on 16 bytes, for %zu (pi_op_prefix_attention_scratch_floats)", what, scratch ? scratch_floats : 0, need); return -1; }
+    A.parts_o = scratch;
+    A.parts_ml = (float2 *) (scratch + (need > 0 ? (size_t) (A.prompt_parts + A.own_parts) * n_tok * n_head * head_dim : 0));
+#define PX_GO(D) px_launch<D>(A, (hipStream_t) stream)
+    return PX_BY_DIM(PX_GO);
+#undef PX_GO
+}
+
+// ---- what cells are given ---------------------------------------------------------------------------------------------------------------------------------------------------------------
+// A wave keeps the keys of 64 cells as operands and the queries of the rows go past it, 64 at a time through LDS for the four waves: a lane has 32 cells of one row of 32, adds their weights up row after row, and the lanes meet at the end.
+struct pm_args {
+    const uint16_t * q; int64_t q_stride;
+    const uint16_t * k; int64_t row;
+    const uint32_t * mask; const float * lse; const int32_t * dyn;
+    float c;
+    int dim, heads, kv, group, n_tok, prompt, n_kv, cell_blocks, row_parts;
+    float decay, * parts, * mass;                            // [row part][key head][cell]; null: the result is whole
+};
+
+template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_mass(const pm_args A, const int32_t * __restrict__ abort_w) {
+    if (pi_aborted(abort_w, 5)) return;
+    constexpr int KS = px_lds<DP>::K, N = DP / 32, CH = DP / 8, STAGE = 64 * KS;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+    __shared__ float lse[2][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
+    const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv), words = (A.n_kv + 31) / 32;
+    const int cb = blockIdx.x % A.cell_blocks, kvh = blockIdx.x / A.cell_blocks % A.kv, part = blockIdx.x / A.cell_blocks / A.kv;
+    const int cells0 = cb * 256, mine = cells0 + wave * 64;
+    if (cells0 >= n_kv) return;                              // (nothing of these cells is read or written: k_mass_merge stops there too)
+    int r0, r1;
+    px_share(A.n_tok * A.group, 64, part, A.row_parts, r0, r1);
+    px_u32x4 key[2][DP / 16], qr[N];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const uint16_t * k = A.k + (int64_t) min(mine + 32 * u + n, n_kv - 1) * A.row + kvh * A.dim;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) key[u][i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (k + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+    }
+    float next_lse = INFINITY;
+    auto load = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int x = i * 256 + tid, d = x % CH * 8, m = min(r + x / CH, r1 - 1);
+            qr[i] = d < A.dim ? *(const px_u32x4 *) (A.q + (int64_t) (m / A.group) * A.q_stride + (int64_t) (kvh * A.group + m % A.group) * A.dim + d) : px_u32x4{ 0, 0, 0, 0 };
+        }
+        if (tid < 64) {
+            const int m = min(r + tid, r1 - 1);
+            const float x = A.lse[(int64_t) (m / A.group) * A.heads + kvh * A.group + m % A.group];
+            next_lse = r + tid >= r1 || x == -INFINITY ? INFINITY : x * 1.44269504f;      // (a row that saw nothing gives nothing)
+        }
+    };
+    auto store = [&](int to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) { const int x = i * 256 + tid; *(px_u32x4 *) (lds + to * STAGE + x / CH * KS + x % CH * 16) = qr[i]; }
+        if (tid < 64) lse[to][tid] = next_lse;
+    };
+    px_f32x16 sum[2] = { px_zero(), px_zero() };
+    const bool masked = cells0 + 256 > prompt;
+    if (r0 < r1) { load(r0); store(0); }
+    int cur = 0;
+    for (int r = r0; r < r1; r += 64, cur ^= 1) {
+        __syncthreads();
+        const bool more = r + 64 < r1;
+        if (more) load(r + 64);
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            if (r + 32 * v >= r1) continue;
+            const uint8_t * qt = lds + cur * STAGE + (32 * v + n) * KS + 16 * g;
+            const float l = lse[cur][32 * v + n];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int base = mine + 32 * u;
+                uint32_t bits = ~0u;
+                if (masked) {
+                    bits = 0;
+                    if (base < n_kv) {
+                        if (base + 32 > prompt) bits = A.mask[(int64_t) (min(r + 32 * v + n, r1 - 1) / A.group) * words + base / 32];
+                        if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
+                        if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
+                    }
+                    if (!__any(bits != 0)) continue;
+                }
+                px_f32x16 s = px_zero();
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) s = px_mfma(key[u][i], *(const px_u32x4 *) (qt + 32 * i), s);
+                if (masked) {
+                    bits >>= 4 * g;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) sum[u][i] += __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -l));
+            }
+        }
+        if (more) store(cur ^ 1);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float x = sum[u][i];
+            x += pi_partner<16>(x); x += pi_partner<8>(x); x += pi_partner<4>(x); x += pi_partner<2>(x); x += pi_partner<1>(x);
+            const int cell = mine + 32 * u + px_cell(i, g);
+            if (n == i && cell < n_kv) {
+                if (A.parts) A.parts[((int64_t) part * A.kv + kvh) * A.n_kv + cell] = x;
+                else A.mass[cell] = A.decay == 0.0f ? x : A.decay * A.mass[cell] + x;
+            }
+        }
+}
+
+__global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, const int32_t * __restrict__ abort_w) {
+    if (pi_aborted(abort_w, 5)) return;
+    const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv;
+    const int64_t cell = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (cell >= n_kv) return;
+    float x = 0.0f;
+    for (int p = 0; p < parts; p++) x += A.parts[(int64_t) p * A.n_kv + cell];
+    A.mass[cell] = A.decay == 0.0f ? x : A.decay * A.mass[cell] + x;
+}
+
+static void pm_plan(pm_args & A) {
+    const int rows = A.n_tok * A.group;
+    A.cell_blocks = (A.n_kv + 255) / 256;
+    A.row_parts = (int) std::max<int64_t>(1, std::min<int64_t>(2 * pi_cu_count() / std::max<int64_t>(1, (int64_t) A.cell_blocks * A.kv), (rows + 63) / 64));
+}
+static size_t pm_floats(const pm_args & A) { const size_t parts = (size_t) A.kv * A.row_parts; return parts > 1 ? parts * A.n_kv : 0; }
+
+extern "C" size_t pi_op_attention_mass_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv) {
+    if (px_sizes("pi_op_attention_mass_scratch_floats", head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0 || n_tok == 0 || n_kv == 0) return 0;
+    pm_args A{};
+    A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.n_kv = n_kv;
+    pm_plan(A);
+    return pm_floats(A);
+}
+
+template <int DP> static int pm_launch(const pm_args & A, hipStream_t s) {
+    const int64_t blocks = (int64_t) A.cell_blocks * A.kv * A.row_parts;
+    if (blocks > 0x7fffffff) { pi_set_error("pi_op_attention_mass: %lld workgroups", (long long) blocks); return -1; }
+    const int nta = std::min(A.n_tok, PI_KT_MAXNT - 1), parts = A.kv * A.row_parts;
+    PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 2.0 * (pi_account_n_kv() > 0 ? pi_account_n_kv() : A.n_kv) * A.row + 2.0 * A.n_tok * A.heads * A.dim, (k_attention_mass<DP>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
+    PI_CHECK_LAUNCH();
+    if (A.parts) {
+        PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 4.0 * A.n_kv * (parts + 2.0), k_mass_merge, dim3((unsigned) A.cell_blocks), dim3(256), 0, s, A, parts, pi_abort_word());
+        PI_CHECK_LAUNCH();
+    }
+    return 0;
+}
+
+extern "C" int pi_op_attention_mass(const uint16_t * q16, int64_t q_stride, const uint16_t * k_cache, const uint32_t * mask, const float * lse, float scale, int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv,
+                                    float decay, float * scratch, size_t scratch_floats, float * mass, const int32_t * dyn, void * stream) {
+    const char * what = "pi_op_attention_mass";
+    if (px_sizes(what, head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0) return -1;
+    if (!std::isfinite(scale) || !std::isfinite(decay)) { pi_set_error("%s: scale %g, decay %g", what, (double) scale, (double) decay); return -1; }
+    if (n_tok == 0 || n_kv == 0) return 0;
+    if (!q16 || !k_cache || !lse || !mass || (!mask && n_kv > n_prompt)) { pi_set_error("%s: queries, keys, lse, mass or mask are NULL", what); return -1; }
+    if (q_stride < (int64_t) n_head * head_dim || q_stride % 8 || (((uintptr_t) q16 | (uintptr_t) k_cache) & 15)) { pi_set_error("%s: rows of queries hold %d heads, %lld values apart (a multiple of 8), queries and keys on 16 bytes", what, n_head, (long long) q_stride); return -1; }
+    pm_args A{};
+    A.q = q16; A.q_stride = q_stride; A.k = k_cache; A.row = (int64_t) n_head_kv * head_dim; A.mask = mask; A.lse = lse; A.dyn = dyn; A.c = scale * 1.44269504f;
+    A.dim = head_dim; A.heads = n_head; A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.prompt = n_prompt; A.n_kv = n_kv; A.decay = decay; A.mass = mass;
+    pm_plan(A);
+    const size_t need = pm_floats(A);
+    if (need > 0 && (!scratch || scratch_floats < need)) { pi_set_error("%s: %zu floats of scratch for %zu (pi_op_attention_mass_scratch_floats)", what, scratch ? scratch_floats : 0, need); return -1; }
+    A.parts = need > 0 ? scratch : nullptr;
+#define PM_GO(D) pm_launch<D>(A, (hipStream_t) stream)
+    return PX_BY_DIM(PM_GO);
+#undef PM_GO
+}

@@ -228,3 +228,12 @@ def _declare(lib):
     lib.pi_op_latent_attention_gated.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, i64, i32, i32, f32, i32, i32, i32, i32, i32, vp, i32, vp, i32, i32, vp, sz, vp, i64, vp, vp]
     lib.pi_op_qkv_prepare_maps.argtypes = [vp, vp, vp, i64, i32, i32, i32, i32, i32, vp, i32, vp, i32, vp, i64, vp, vp, vp, vp, vp]
     lib.pi_op_diff_attention.argtypes = [vp, i64, vp, vp, vp, vp, vp, f32, i32, i32, i32, f32, f32, f32, i32, i32, i32, i32, i32, i32, vp, sz, vp, i64, vp, vp]
+    # continuations of one prompt: attention over shared cells, what cells are given, cuts of a cache, sampling
+    lib.pi_op_prefix_attention.argtypes = [vp, i64, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, vp, sz, vp, i64, vp, vp, vp]
+    lib.pi_op_prefix_attention_scratch_floats.argtypes = [i32, i32, i32, i32, i32, i32]; lib.pi_op_prefix_attention_scratch_floats.restype = sz
+    lib.pi_op_attention_mass.argtypes = [vp, i64, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, f32, vp, sz, vp, vp, vp]
+    lib.pi_op_attention_mass_scratch_floats.argtypes = [i32, i32, i32, i32, i32, i32]; lib.pi_op_attention_mass_scratch_floats.restype = sz
+    lib.pi_op_cache_choose.argtypes = [vp, vp, i32, i32, vp, vp]
+    lib.pi_op_cache_move.argtypes = [vp, vp, i32, vp, i32, i32, vp]
+    lib.pi_op_sample.argtypes = [vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, sz, vp, vp, vp, vp]
+    lib.pi_op_sample_scratch_bytes.argtypes = [i32, i32]; lib.pi_op_sample_scratch_bytes.restype = sz

@@ -1,0 +1,531 @@
+"""Operators of a batch of continuations of one prompt (prefix_attention.hip, cache_cut.hip, sampling.hip): attention over shared cells, what cells are given, cuts of a cache, sampling.  Against their definitions in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from pipeinfer_amd import lib as L
+
+P = 4096                                                                       # an address that no refused call looks at
+
+
+def attention_call(lib, q=P, stride=None, k=P, v=P, mask=P, scale=0.1, dim=64, heads=8, kv=2, tok=3, prompt=100, n=140, scratch=P, floats=1 << 40, out=P, out_stride=None, lse=None, dyn=None, stream=None):
+    return lib.pi_op_prefix_attention(q, heads * dim if stride is None else stride, k, v, mask, scale, dim, heads, kv, tok, prompt, n, scratch, floats, out, heads * dim if out_stride is None else out_stride, lse, dyn, stream)
+
+
+@pytest.mark.parametrize("args,why", [
+    (dict(dim=60), b"8 .. 256 values in steps of 8"), (dict(dim=264), b"8 .. 256"), (dict(dim=0), b"8 .. 256"), (dict(kv=3), b"whole groups"), (dict(heads=0), b"0 query heads"), (dict(kv=0), b"over 0 key"),
+    (dict(tok=-1), b"-1 tokens"), (dict(prompt=141), b"141 of 140 cells"), (dict(prompt=-1), b"-1 of 140"), (dict(scale=0.0), b"scale 0"), (dict(scale=-1.0), b"scale -1"), (dict(scale=float("nan")), b"scale"),
+    (dict(scale=float("inf")), b"scale"), (dict(q=None), b"are NULL"), (dict(k=None), b"are NULL"), (dict(v=None), b"are NULL"), (dict(out=None), b"are NULL"), (dict(mask=None), b"are NULL"), (dict(stride=504), b"504"),
+    (dict(stride=516), b"516"), (dict(out_stride=508), b"508"), (dict(out_stride=514), b"514"), (dict(q=P + 8), b"16 bytes"), (dict(k=P + 2), b"16 bytes"), (dict(v=P + 4), b"16 bytes"), (dict(out=P + 4), b"16 bytes"),
+    (dict(scratch=None), b"0 floats of scratch"), (dict(floats=10), b"10 floats of scratch"), (dict(scratch=P + 8), b"on 16 bytes, for"),
+])
+def test_attention_refuses(args, why):
+    lib = L.load()
+    assert attention_call(lib, **args) != 0 and why in lib.pi_last_error(), lib.pi_last_error()
+
+
+@pytest.mark.parametrize("call,why", [
+    (lambda lib, mass: mass(dim=12), b"steps of 8"), (lambda lib, mass: mass(prompt=500), b"500 of"), (lambda lib, mass: mass(lse=None), b"are NULL"), (lambda lib, mass: mass(mass=None), b"are NULL"),
+    (lambda lib, mass: mass(k=None), b"are NULL"), (lambda lib, mass: mass(mask=None), b"are NULL"), (lambda lib, mass: mass(q=P + 2), b"16 bytes"), (lambda lib, mass: mass(stride=511), b"511"), (lambda lib, mass: mass(decay=float("nan")), b"decay"),
+    (lambda lib, mass: mass(scale=float("inf")), b"scale"), (lambda lib, mass: mass(scratch=None), b"0 floats"), (lambda lib, mass: mass(floats=3), b"3 floats"),
+    (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 11, P, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, -1, P, None), b"-1 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(None, None, 10, 4, P, None), b"is NULL"),
+    (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 4, None, None), b"is NULL"),
+    (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, P, 11, 10, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_move(None, None, 1, P, 4, 10, None), b"is NULL"),
+    (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(0), (C.c_int64 * 1)(16), 1, P, 4, 10, None), b"array 0 is NULL"), (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(0), 1, P, 4, 10, None), b"rows of 0 bytes"),
+    (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, None, 4, 10, None), b"is NULL"), (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), -1, P, 4, 10, None), b"-1 arrays"),
+    (lambda lib, mass: lib.pi_op_sample(P, 99, 100, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"99 apart"), (lambda lib, mass: lib.pi_op_sample(P, 100, 0, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"1 .. 524288"),
+    (lambda lib, mass: lib.pi_op_sample(P, 1 << 20, 1 << 20, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"1 .. 524288"), (lambda lib, mass: lib.pi_op_sample(P, 100, 100, -1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"-1 rows"),
+    (lambda lib, mass: lib.pi_op_sample(None, 100, 100, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"are NULL"), (lambda lib, mass: lib.pi_op_sample(P, 100, 100, 1, P, P, P, P, None, P, 1 << 30, P, P, P, None), b"are NULL"),
+    (lambda lib, mass: lib.pi_op_sample(P, 100, 100, 1, P, P, P, P, P, P, 1 << 30, None, P, P, None), b"are NULL"),
+])
+def test_the_others_refuse(call, why):
+    lib = L.load()
+
+    def mass(q=P, stride=512, k=P, mask=P, lse=P, scale=0.1, dim=64, heads=8, kv=2, tok=3, prompt=100, n=140, decay=1.0, scratch=P, floats=1 << 40, mass=P, dyn=None):
+        return lib.pi_op_attention_mass(q, stride, k, mask, lse, scale, dim, heads, kv, tok, prompt, n, decay, scratch, floats, mass, dyn, None)
+
+    assert call(lib, mass) != 0 and why in lib.pi_last_error(), lib.pi_last_error()
+
+
+def test_nothing_to_do_is_no_error():
+    """no tokens, no rows, no arrays, nothing kept or nothing given up: done without a launch (none would succeed here)"""
+    lib = L.load()
+    assert attention_call(lib, tok=0) == 0 and lib.pi_op_sample(P, 100, 100, 0, P, P, P, P, P, P, 0, P, P, P, None) == 0 and lib.pi_op_cache_choose(P, None, 10, 0, P, None) == 0
+    one, size = (C.c_void_p * 1)(P), (C.c_int64 * 1)(16)
+    assert lib.pi_op_cache_move(one, size, 0, P, 4, 10, None) == 0 and lib.pi_op_cache_move(one, size, 1, P, 0, 10, None) == 0 and lib.pi_op_cache_move(one, size, 1, P, 10, 10, None) == 0
+    assert lib.pi_op_attention_mass(P, 512, P, P, P, 0.1, 64, 8, 2, 0, 100, 140, 1.0, P, 1 << 40, P, None, None) == 0
+
+
+# ---- on the GPU --------------------------------------------------------------------------------------------------------------------------------------------------------------------
+def gpu():
+    from tests import gpu_util as U
+    return U, U.init()
+
+
+def pack(seen):
+    """[rows][cells] truth values as a bitmap, 32 cells to a word"""
+    t, n = seen.shape
+    bits = np.zeros((t, (n + 31) // 32 * 32), np.uint8)
+    bits[:, :n] = seen
+    return np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view(np.uint32)
+
+
+def soft_max(q, k, v, seen, scale):
+    """out, lse and the weights, [tokens][heads][..], from the definition"""
+    T, H, D = q.shape
+    per = H // k.shape[1]
+    q, k, v = (x.astype(np.float64) for x in (q, k, v))
+    out, lse, p = np.zeros((T, H, D)), np.full((T, H), -np.inf), np.zeros((T, H, k.shape[0]))
+    for t in range(T):
+        c = np.flatnonzero(seen[t])
+        if len(c) == 0:
+            continue
+        for h in range(H):
+            s = k[c, h // per] @ q[t, h] * scale
+            m = s.max()
+            lse[t, h] = m + np.log(np.exp(s - m).sum())
+            p[t, h, c] = np.exp(s - lse[t, h])
+            out[t, h] = p[t, h, c] @ v[c, h // per]
+    return out, lse, p
+
+
+def inputs(rng, heads, kv, dim, tokens, prompt, own, spread=2.0, loners=True):
+    """caches with rows behind the last cell that no call may look at, what nobody sees being no number; token t sees its own cells, the last token no cell behind the prompt"""
+    n = prompt + own
+    q = (spread * rng.standard_normal((tokens, heads, dim))).astype(np.float16)
+    k, v = (rng.standard_normal((n + 5, kv, dim)).astype(np.float16) for _ in range(2))
+    seen = np.zeros((tokens, n), bool)
+    seen[:, :prompt] = True
+    seen[:, prompt:] = rng.random((tokens, own)) < min(1.0, 1.5 / tokens + 0.05)
+    if loners:
+        seen[-1, prompt:] = False
+    nobody = np.append(~seen.any(0), [True] * 5)
+    k[nobody], v[nobody] = np.nan, np.inf
+    return q, k, v, seen
+
+
+class Pass:
+    """one pass's arrays on the device and its calls; rows of queries and outputs lie further apart than they are long"""
+
+    def __init__(self, U, lib, q, k, v, seen, prompt, scale, room=None):
+        self.lib, self.U = lib, U
+        self.T, self.H, self.D = q.shape
+        self.KH, self.prompt, self.n, self.scale = k.shape[1], prompt, seen.shape[1], scale
+        self.qs, self.os = self.H * self.D + 8, self.H * self.D + 4
+        rows = np.full((self.T, self.qs), np.nan, np.float16)
+        rows[:, :self.H * self.D] = q.reshape(self.T, -1)
+        self.room = (prompt, self.n) if room is None else room          # what the arguments say where the device says less
+        mask = np.zeros((self.T, max(self.room[1], self.n)), bool)
+        mask[:, :self.n] = seen
+        mask[:, :prompt] = False                                         # (not looked at)
+        self.q, self.k, self.v, self.mask = U.Dev(rows), U.Dev(k), U.Dev(v), U.Dev(pack(mask))
+        self.out, self.lse = U.Dev(np.full((self.T, self.os), 7.0, np.float32)), U.Dev(np.full((self.T, self.H), 7.0, np.float32))
+        self.dyn = None if room is None else U.Dev(np.array([prompt, self.n], np.int32))
+        sizes = (self.D, self.H, self.KH, self.T) + self.room
+        self.floats, self.mass_floats = lib.pi_op_prefix_attention_scratch_floats(*sizes), lib.pi_op_attention_mass_scratch_floats(*sizes)
+        self.scratch = U.Dev(np.full(max(self.floats, self.mass_floats) + 4, np.nan, np.float32))
+
+    def attend(self, stream=None):
+        L.check(self.lib.pi_op_prefix_attention(self.q.ptr, self.qs, self.k.ptr, self.v.ptr, self.mask.ptr, self.scale, self.D, self.H, self.KH, self.T, *self.room, self.scratch.ptr, self.floats, self.out.ptr, self.os, self.lse.ptr,
+                                                self.dyn and self.dyn.ptr, stream), "pi_op_prefix_attention")
+
+    def give(self, mass, decay, stream=None):
+        L.check(self.lib.pi_op_attention_mass(self.q.ptr, self.qs, self.k.ptr, self.mask.ptr, self.lse.ptr, self.scale, self.D, self.H, self.KH, self.T, *self.room, decay, self.scratch.ptr, self.mass_floats, mass.ptr,
+                                              self.dyn and self.dyn.ptr, stream), "pi_op_attention_mass")
+
+    def outputs(self):
+        out = self.out.get(np.float32, (self.T, self.os))
+        assert (out[:, self.H * self.D:] == 7.0).all()
+        assert np.isnan(self.scratch.get(np.float32)[max(self.floats, self.mass_floats):]).all()
+        return out[:, :self.H * self.D].reshape(self.T, self.H, self.D), self.lse.get(np.float32, (self.T, self.H))
+
+
+# A weight's relative error: the score s scale log2(e), |.| < 2^5 here, is rounded at 2^-24 of itself three times (the sum of products, the factor, the difference): 3 x 2^-20 ln 2 = 2e-6 at most, the exponential 2^-23, its two halves 2^-22.
+# Sums of n terms in fp32, a few partial sums each of at most 2^11: random signs, 2^-24 x 2^5.5.  An output's error relative to the outputs' size is below the weights' worst one: 4e-6 in the 2-norm
+FAR, LSE_FAR = 4e-6, 1e-5
+
+
+def check_attention(got, want, lse, want_lse):
+    assert np.isfinite(got).all()
+    assert np.linalg.norm(got - want) <= FAR * np.linalg.norm(want) + 1e-30
+    none = np.isneginf(want_lse)
+    assert (np.isneginf(lse) == none).all() and (got[none] == 0).all()
+    assert np.abs(lse[~none] - want_lse[~none]).max(initial=0.0) <= LSE_FAR                # (at most 2^4: its own rounding is 2^-21, the sum's and the logarithm's as much)
+
+
+SIZES = [(1, 1, 8, 1, 1, 0), (1, 1, 8, 1, 0, 1), (2, 1, 8, 2, 31, 3), (32, 4, 64, 1, 500, 13), (4, 4, 128, 24, 100, 70), (8, 1, 128, 16, 129, 40), (64, 8, 128, 3, 1000, 33), (71, 1, 64, 2, 65, 90), (71, 1, 64, 1, 0, 700), (6, 2, 40, 33, 64, 1),
+         (3, 3, 80, 5, 300, 0), (24, 3, 96, 9, 1, 257), (8, 2, 256, 7, 90, 63), (8, 2, 256, 17, 400, 64), (5, 1, 24, 20, 777, 500), (4, 2, 192, 40, 333, 31), (2, 2, 160, 2, 0, 0), (9, 3, 72, 30, 0, 200), (16, 2, 64, 8, 4096, 64), (4, 1, 32, 64, 2000, 9000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", SIZES)
+def test_attention(heads, kv, dim, tokens, prompt, own):
+    """one token to many, heads with keys of their own to 71 over one, nothing shared, nothing but shared, cells that are no multiple of anything, a token that sees nothing"""
+    U, lib = gpu()
+    rng = np.random.default_rng(heads * 1000 + tokens)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own)
+    p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5)
+    p.attend()
+    got, lse = p.outputs()
+    want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
+    check_attention(got, want, lse, want_lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(32, 4, 64, 4, 500, 40), (8, 2, 128, 50, 300, 100)])
+def test_sizes_on_the_device(heads, kv, dim, tokens, prompt, own):
+    """room for more cells than there are: the device says how many are shared and live; parts without a cell count for nothing, and the mass of what is not live stays"""
+    U, lib = gpu()
+    rng = np.random.default_rng(tokens)
+    for share, live in ((prompt, own), (0, own), (prompt, 0), (prompt // 3, 2 * own), (0, 0)):
+        q, k, v, seen = inputs(rng, heads, kv, dim, tokens, share, live)
+        room = (4000, 9000)
+        k, v = (np.concatenate([x, np.full((room[1] - len(x), kv, dim), np.nan, np.float16)]) for x in (k, v))
+        p = Pass(U, lib, q, k, v, seen, share, dim ** -0.5, room)
+        p.attend()
+        got, lse = p.outputs()
+        want, want_lse, w = soft_max(q, k, v, seen, dim ** -0.5)
+        check_attention(got, want, lse, want_lse)
+        mass = U.Dev(np.full(room[1], 3.0, np.float32))
+        p.give(mass, 0.5)
+        m = mass.get(np.float32)
+        n = share + live
+        assert (m[n:] == 3.0).all() and np.allclose(m[:n], 1.5 + w.sum((0, 1))[:n], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_scores_far_apart():
+    """scores that grow along the cells by far more than the maximum may lag, that fall, and that are huge: the sums are relative to the right maximum"""
+    U, lib = gpu()
+    rng = np.random.default_rng(5)
+    for tokens in (2, 40):
+        for slope in (0.5, -0.5, 40.0):
+            q, k, v, seen = inputs(rng, 4, 1, 64, tokens, 700, 50)
+            q[...] = 1.0
+            k[:750] = (np.arange(750)[:, None, None] * (slope / 64)).astype(np.float16)
+            v[:750] = rng.standard_normal((750, 1, 64)).astype(np.float16)
+            p = Pass(U, lib, q, k, v, seen, 700, 1.0)
+            p.attend()
+            got, lse = p.outputs()
+            want, want_lse, _ = soft_max(q, k, v, seen, 1.0)
+            # (scores of up to 2^15: the sum of products is exact, the factor log2(e) is rounded at 2^-24 of it: 2^-9 x ln 2 of a weight, and of the lse)
+            far = 2 ** -24 * 3 * max(1.0, np.abs(want_lse[np.isfinite(want_lse)]).max())
+            assert np.linalg.norm(got - want) <= max(FAR, far) * np.linalg.norm(want) and np.abs(lse - want_lse).max() <= max(LSE_FAR, far)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", SIZES)
+def test_mass(heads, kv, dim, tokens, prompt, own):
+    """what the cells are given adds up to the rows that see anything; the old mass fades, or is not looked at"""
+    U, lib = gpu()
+    rng = np.random.default_rng(heads * 1000 + tokens + 1)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own)
+    n, scale = prompt + own, dim ** -0.5
+    if n == 0:
+        return
+    p = Pass(U, lib, q, k, v, seen, prompt, scale)
+    _, want_lse, w = soft_max(q, k, v, seen, scale)
+    p.lse = U.Dev(want_lse.astype(np.float32))
+    old = rng.random(n + 3).astype(np.float32)
+    given = w.sum((0, 1))[:n]
+    for decay, before in ((1.0, old), (0.25, old), (0.0, np.full(n + 3, np.nan, np.float32))):
+        mass = U.Dev(before)
+        p.give(mass, decay)
+        got = mass.get(np.float32)
+        want = given + (decay * before[:n].astype(np.float64) if decay else 0.0)
+        # (a weight as in FAR, and the lse's own rounding, 2^-21; all terms are positive)
+        assert np.allclose(got[:n], want, rtol=8e-6, atol=1e-12), (decay, np.abs(got[:n] / want - 1).max())
+        assert np.array_equal(got[n:], before[n:], equal_nan=True)
+
+
+def chosen(mass, guarded, keep):
+    order = sorted(range(len(mass)), key=lambda i: (0, 0, 0, i) if guarded[i] else (1, np.isnan(mass[i]), 0 if np.isnan(mass[i]) else -mass[i], i))[:keep]
+    stays = set(order)
+    movers = iter(sorted(i for i in order if i >= keep))
+    return np.array([i if i in stays else next(movers) for i in range(keep)], np.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cells", [1, 2, 63, 65, 1000, 4097, 20000, 33000, 100001])
+def test_choice(cells):
+    """masses of every kind: spread, all equal, few different ones, signs, infinities and what is no number; guards, more of them than stay; one cell to all of them"""
+    U, lib = gpu()
+    rng = np.random.default_rng(cells)
+    kinds = {"spread": rng.random(cells) ** 4 * 50, "equal": np.full(cells, 2.5), "few": rng.integers(0, 3, cells) * 0.5, "signs": np.where(rng.random(cells) < 0.3, -0.0, rng.standard_normal(cells)),
+             "odd": np.where(rng.random(cells) < 0.2, np.nan, np.where(rng.random(cells) < 0.2, np.inf, np.where(rng.random(cells) < 0.2, -np.inf, rng.standard_normal(cells)))), "zeros": np.where(rng.random(cells) < 0.5, 0.0, -0.0)}
+    for name, mass in kinds.items():
+        mass = mass.astype(np.float32)
+        for keep in sorted({1, cells // 3, cells // 2 + 1, cells - 1, cells} - {0} if cells < 30000 else {cells // 2, 5, cells - 7}):
+            if keep == 0:
+                continue
+            for guards in (None, 0.05, 0.9):
+                guarded = np.zeros(cells, bool) if guards is None else rng.random(cells) < guards
+                m, g, s = U.Dev(mass), U.Dev(pack(guarded[None])), U.Dev(np.full(keep + 1, -9, np.int32))
+                L.check(lib.pi_op_cache_choose(m.ptr, None if guards is None else g.ptr, cells, keep, s.ptr, None), "pi_op_cache_choose")
+                got = s.get(np.int32)
+                assert np.array_equal(got[:keep], chosen(mass, guarded, keep)) and got[keep] == -9, (name, keep, guards)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cells,keep,sizes", [(1000, 700, [4, 512, 2064, 6, 1, 16384, 12]), (300, 20, [2048] * 130 + [4]), (5000, 2500, [160, 80, 4])])
+def test_rows_that_move(cells, keep, sizes):
+    """rows of every alignment, more arrays than a launch takes; entries that point in front of the budget or behind the cache move nothing"""
+    U, lib = gpu()
+    rng = np.random.default_rng(cells)
+    source = chosen(rng.random(cells), np.zeros(cells, bool), keep)
+    odd = rng.permutation(keep)[:3]
+    source[odd] = [0, -5, cells]
+    arrays = [rng.integers(0, 256, (cells, b), np.uint8) for b in sizes]
+    dev, s = [U.Dev(a) for a in arrays], U.Dev(source)
+    at, size = (C.c_void_p * len(dev))(*[d.ptr for d in dev]), (C.c_int64 * len(dev))(*sizes)
+    L.check(lib.pi_op_cache_move(at, size, len(dev), s.ptr, keep, cells, None), "pi_op_cache_move")
+    for d, a in zip(dev, arrays):
+        want = a.copy()
+        for i, c in enumerate(source):
+            if keep <= c < cells:
+                want[i] = a[c]
+        assert np.array_equal(d.get(np.uint8, a.shape), want)
+
+
+def sampled(x, temp, top_k, top_p, min_p, u):
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    order = np.argsort(-x, kind="stable")
+    order = order[x[order] > -np.inf]
+    if len(order) == 0:
+        return -1, 0.0, 0, True
+    top = x[order[0]]
+
+    def below(v):
+        return np.where(v == top, 0.0, v - top)
+
+    if top_k > 0:
+        order = order[:top_k]
+    w = np.exp(below(x[order]))
+    sure = True
+    if top_p < 1:
+        ahead = np.cumsum(w) - w
+        edge = np.float64(top_p) * w.sum()
+        n = max(1, int((ahead < edge).sum()))
+        near = np.abs(ahead / edge - 1).min() if edge > 0 else 1.0
+        sure &= bool(near > 1e-9 or top_p <= 0)
+        order, w = order[:n], w[:n]
+    n = max(1, int((w >= np.float64(min_p)).sum())) if min_p > 0 else len(order)
+    order = order[:n]
+    if not temp > 0:
+        return order[0], 1.0, n, sure
+    ids = np.sort(order)
+    e = np.exp(below(x[ids]) / np.float64(temp))
+    cum = np.cumsum(np.floor(e * 2.0 ** 44 + 0.5))                      # (the steps in which sums are held: weights below half of one are never drawn)
+    i = int(np.searchsorted(cum, np.float64(u) * cum[-1], side="right"))
+    sure &= bool(np.abs(cum / cum[-1] - u).min() > 1e-9 or u == 0)
+    cum = np.cumsum(e)
+    return ids[i], e[i] / cum[-1], n, sure
+
+
+def run_sample(U, lib, x, vocab, settings, u):
+    """rows as they are in memory (x: [rows][stride])"""
+    rows = len(x)
+    size = lib.pi_op_sample_scratch_bytes(vocab, rows)
+    d, scratch = U.Dev(x), U.Dev(nbytes=size + 16)
+    dev = [None if s is None else U.Dev(np.asarray(s, t)) for s, t in zip(settings, (np.float32, np.int32, np.float32, np.float32))]
+    du, out = U.Dev(np.asarray(u, np.float32)), [U.Dev(np.full(rows, -7, t)) for t in (np.int32, np.float32, np.int32)]
+    L.check(lib.pi_op_sample(d.ptr, x.shape[1], vocab, rows, *[s and s.ptr for s in dev], du.ptr, scratch.ptr, size, *[o.ptr for o in out], None), "pi_op_sample")
+    return [o.get(t) for o, t in zip(out, (np.int32, np.float32, np.int32))]
+
+
+def check_sample(U, lib, x, vocab, settings, u):
+    got = run_sample(U, lib, x, vocab, settings, u)
+    full = [np.full(len(x), v) if s is None else np.asarray(s) for s, v in zip(settings, (1.0, 0, 1.0, 0.0))]
+    for t in range(len(x)):
+        i, p, n, sure = sampled(x[t, :vocab], np.float32(full[0][t]), int(full[1][t]), np.float32(full[2][t]), np.float32(full[3][t]), np.float32(u[t]))
+        assert sure, ("an input at a border", t)                         # (no test asks which side of a border a sum falls that two roundings could move)
+        assert got[0][t] == i and got[2][t] == n and abs(got[1][t] - p) <= 2.0 ** -23 * p, (t, [f[t] for f in full], u[t], got[0][t], i, got[2][t], n, got[1][t], p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,stride", [(1, 1), (3, 7), (300, 300), (1000, 1004), (8191, 8191), (32000, 32000), (32001, 32003), (131072, 131072), (262144, 262144), (300001, 300001)])
+def test_sample(vocab, stride):
+    """every setting by itself and together, the smallest vocabulary to more than most have, rows that begin anywhere"""
+    U, lib = gpu()
+    rng = np.random.default_rng(vocab)
+    rows = 24 if vocab < 100000 else 8
+    for spread in (2.5, 8.0):
+        x = np.full((rows, stride), np.nan, np.float32)
+        x[:, :vocab] = spread * rng.standard_normal((rows, vocab))
+        x[::3, :vocab][rng.random(x[::3, :vocab].shape) < 0.6] = -np.inf
+        x[:, vocab:] = 100.0
+        u = rng.random(rows)
+        check_sample(U, lib, x, vocab, (None, None, None, None), u)
+        check_sample(U, lib, x, vocab, (np.full(rows, 0.7), np.full(rows, 40), None, None), u)
+        check_sample(U, lib, x, vocab, (np.full(rows, 1.3), None, np.full(rows, 0.9), None), u)
+        check_sample(U, lib, x, vocab, (None, None, None, np.full(rows, 0.05)), u)
+        check_sample(U, lib, x, vocab, (rng.choice([0.0, 0.5, 1.0, 2.0, -1.0], rows), rng.choice([0, 1, 2, 50, 128, 129, 1000, 200000, -3], rows), rng.choice([0.0, 0.3, 0.8, 0.99, 1.0, 2.0], rows), rng.choice([0.0, 0.02, 0.3, 1.0], rows)), u)
+
+
+@pytest.mark.gpu
+def test_sample_of_odd_rows():
+    """rows of equal logits (the border inside them goes by the id), of few values, of nothing, with infinities and what is no number, one logit far above; the ends of u"""
+    U, lib = gpu()
+    rng = np.random.default_rng(3)
+    V = 40000
+    x = np.zeros((12, V), np.float32)
+    x[1] = rng.integers(-3, 3, V)
+    x[2] = -np.inf
+    x[3] = np.nan
+    x[4] = rng.standard_normal(V); x[4, [7, 900, 39999]] = np.inf
+    x[5] = rng.standard_normal(V); x[5, ::2] = np.nan
+    x[6] = rng.standard_normal(V); x[6, 123] = 500.0
+    x[7] = -np.inf; x[7, 31111] = -3e38
+    x[8] = np.where(rng.random(V) < 0.5, 0.0, -0.0)
+    x[9] = 1e-30 * rng.standard_normal(V)
+    x[10] = 3e38 * np.clip(rng.standard_normal(V), -1, 1)
+    x[11] = np.sort(3 * rng.standard_normal(V))
+    rows = len(x)
+    for u in (0.0, 0.3, 0.777, 1 - 2.0 ** -24):
+        for settings in ((None, None, None, None), (np.full(rows, 0.5), np.full(rows, 100), np.full(rows, 0.3), None), (None, np.full(rows, 777), None, None), (None, np.full(rows, 777), np.full(rows, 0.4321), np.full(rows, 0.5)),
+                         (None, None, np.full(rows, 0.6543), None), (np.zeros(rows), None, np.full(rows, 0.2), None), (np.full(rows, np.inf), None, None, np.full(rows, 0.01)), (np.full(rows, 1e-3), np.full(rows, 3), None, None)):
+            got = run_sample(U, lib, x, V, settings, [u] * rows)
+            full = [np.full(rows, v) if s is None else np.asarray(s) for s, v in zip(settings, (1.0, 0, 1.0, 0.0))]
+            for t in range(rows):
+                with np.errstate(invalid="ignore"):
+                    i, p, n, sure = sampled(x[t], np.float32(full[0][t]), int(full[1][t]), np.float32(full[2][t]), np.float32(full[3][t]), np.float32(u))
+                if not sure:                                                 # (equal weights put borders on whole counts: u x 40000 may be one.  Then the neighbour is as right)
+                    assert abs(int(got[2][t]) - n) <= 1 and abs(got[1][t] - p) <= 1e-4 * p, (t, u)
+                    continue
+                assert got[0][t] == i and got[2][t] == n and abs(got[1][t] - p) <= 2.0 ** -23 * p, (t, u, got[0][t], i, got[2][t], n, got[1][t], p)
+
+
+@pytest.mark.gpu
+def test_outputs_that_nobody_wants():
+    U, lib = gpu()
+    rng = np.random.default_rng(8)
+    x, ids = U.Dev(rng.standard_normal((3, 500)).astype(np.float32)), [U.Dev(np.zeros(3, np.int32)) for _ in range(2)]
+    prob, kept, u = U.Dev(np.zeros(3, np.float32)), U.Dev(np.zeros(3, np.int32)), U.Dev(np.full(3, 0.4, np.float32))
+    size = lib.pi_op_sample_scratch_bytes(500, 3)
+    scratch = U.Dev(nbytes=size + 16)
+    L.check(lib.pi_op_sample(x.ptr, 500, 500, 3, None, None, None, None, u.ptr, scratch.ptr, size, ids[0].ptr, None, None, None), "pi_op_sample")
+    L.check(lib.pi_op_sample(x.ptr, 500, 500, 3, None, None, None, None, u.ptr, scratch.ptr, size, ids[1].ptr, prob.ptr, kept.ptr, None), "pi_op_sample")
+    assert np.array_equal(ids[0].get(np.int32), ids[1].get(np.int32)) and (kept.get(np.int32) == 500).all()
+    q, k, v, seen = inputs(rng, 4, 2, 64, 3, 50, 20)
+    p = Pass(U, lib, q, k, v, seen, 50, 0.125)
+    p.attend()
+    want, _ = p.outputs()
+    p.out = U.Dev(np.full((3, p.os), 7.0, np.float32))
+    L.check(lib.pi_op_prefix_attention(p.q.ptr, p.qs, p.k.ptr, p.v.ptr, p.mask.ptr, p.scale, 64, 4, 2, 3, 50, 70, p.scratch.ptr, p.floats, p.out.ptr, p.os, None, None, None), "pi_op_prefix_attention")
+    assert np.array_equal(p.outputs()[0], want)
+
+
+@pytest.mark.gpu
+def test_a_serving_step():
+    """as they are used together: attention, what the cells were given, a cut of the caches, attention over what is left - the same as over the kept cells from the start -, and a token for every row"""
+    U, lib = gpu()
+    rng = np.random.default_rng(77)
+    heads, kv, dim, tokens, prompt, own, scale = 16, 2, 64, 12, 700, 60, 0.125
+    n, keep = prompt + own, 400
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own, loners=False)
+    k[n:], v[n:] = 0, 0
+    bad = ~seen.any(0)
+    k[:n][bad], v[:n][bad] = 0, 0
+    p = Pass(U, lib, q, k, v, seen, prompt, scale)
+    mass = U.Dev(np.zeros(n, np.float32))
+    guarded = np.zeros(n, bool)
+    guarded[prompt:] = True                                              # the continuations' own cells and the prompt's first
+    guarded[:4] = True
+    guard, source, pos = U.Dev(pack(guarded[None])), U.Dev(np.zeros(keep, np.int32)), U.Dev(np.arange(n, dtype=np.int32))
+    p.attend()
+    p.give(mass, 1.0)
+    L.check(lib.pi_op_cache_choose(mass.ptr, guard.ptr, n, keep, source.ptr, None), "pi_op_cache_choose")
+    arrays = (C.c_void_p * 3)(p.k.ptr, p.v.ptr, pos.ptr)
+    L.check(lib.pi_op_cache_move(arrays, (C.c_int64 * 3)(2 * kv * dim, 2 * kv * dim, 4), 3, source.ptr, keep, n, None), "pi_op_cache_move")
+    _, _, w = soft_max(q, k, v, seen, scale)
+    got_mass, src = mass.get(np.float32), source.get(np.int32)
+    assert np.allclose(got_mass, w.sum((0, 1))[:n], rtol=1e-5, atol=1e-9)
+    assert np.array_equal(src, chosen(got_mass, guarded, keep)) and np.array_equal(pos.get(np.int32)[:keep], src)
+    # the kept cells' mask; how many of them in front everybody still sees
+    left = seen[:, src]
+    shared = int(np.argmin(left.all(0))) if not left.all() else keep
+    after = Pass(U, lib, q, p.k.get(np.float16, k.shape)[:keep + 5], p.v.get(np.float16, v.shape)[:keep + 5], left, shared, scale)
+    after.attend()
+    out, lse = after.outputs()
+    want, want_lse, _ = soft_max(q, k[src], v[src], left, scale)
+    check_attention(out, want, lse, want_lse)
+    check_sample(U, lib, out.reshape(tokens, -1) * 20, heads * dim, (np.full(tokens, 0.8), np.full(tokens, 40), np.full(tokens, 0.95), np.full(tokens, 0.01)), rng.random(tokens))
+
+
+class Hip:
+    """streams and graphs of the runtime that the library runs on"""
+
+    def __init__(self):
+        self.hip = C.CDLL("libamdhip64.so.7")
+        for name in ("hipStreamCreate", "hipStreamDestroy", "hipStreamBeginCapture", "hipStreamEndCapture", "hipGraphInstantiate", "hipGraphLaunch", "hipGraphExecDestroy", "hipGraphDestroy"):
+            getattr(self.hip, name).restype = C.c_int
+
+    def stream(self):
+        s = C.c_void_p()
+        assert self.hip.hipStreamCreate(C.byref(s)) == 0
+        return s.value
+
+    def capture(self, stream, work):
+        graph, run = C.c_void_p(), C.c_void_p()
+        assert self.hip.hipStreamBeginCapture(C.c_void_p(stream), 0) == 0
+        work()
+        assert self.hip.hipStreamEndCapture(C.c_void_p(stream), C.byref(graph)) == 0
+        assert self.hip.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+        return run
+
+    def replay(self, run, stream):
+        assert self.hip.hipGraphLaunch(run, C.c_void_p(stream)) == 0
+
+
+@pytest.mark.gpu
+def test_captured_and_beside_each_other():
+    """two passes on two streams with scratch of their own, and the whole step in a graph that is replayed with eager work between: the same bits each time"""
+    U, lib = gpu()
+    rng = np.random.default_rng(6)
+    hip = Hip()
+    passes, streams = [], [hip.stream() for _ in range(2)]
+    for seed in range(2):
+        q, k, v, seen = inputs(rng, 16, 2, 128, 20, 900, 130)
+        p = Pass(U, lib, q, k, v, seen, 900, 0.09)
+        x = rng.standard_normal((20, 50000)).astype(np.float32) * 3
+        p.x, p.u, p.tk, p.tp = U.Dev(x), U.Dev(rng.random(20).astype(np.float32)), U.Dev(np.array([0, 50] * 10, np.int32)), U.Dev(np.full(20, 0.9, np.float32))
+        p.size = lib.pi_op_sample_scratch_bytes(50000, 20)
+        p.room_s, p.id, p.prob, p.kept = U.Dev(nbytes=p.size + 16), *[U.Dev(np.zeros(20, np.int32)) for _ in range(3)]
+        p.mass, p.source = U.Dev(np.zeros(1030, np.float32)), U.Dev(np.zeros(500, np.int32))
+        passes.append(p)
+
+    def step(p, stream):
+        p.attend(stream)
+        p.give(p.mass, 0.0, stream)
+        L.check(lib.pi_op_cache_choose(p.mass.ptr, None, 1030, 500, p.source.ptr, stream), "pi_op_cache_choose")
+        L.check(lib.pi_op_sample(p.x.ptr, 50000, 50000, 20, None, p.tk.ptr, p.tp.ptr, None, p.u.ptr, p.room_s.ptr, p.size, p.id.ptr, p.prob.ptr, p.kept.ptr, stream), "pi_op_sample")
+
+    def results(p):
+        out, lse = p.outputs()
+        return [out, lse, p.mass.get(np.float32), p.source.get(np.int32), p.id.get(np.int32), p.prob.get(np.float32), p.kept.get(np.int32)]
+
+    alone = []
+    for p in passes:
+        step(p, None)
+        alone.append(results(p))
+    L.check(lib.pi_device_sync(), "sync")
+    for _ in range(5):
+        for p, s in zip(passes, streams):
+            step(p, s)
+    L.check(lib.pi_device_sync(), "sync")
+    for p, want in zip(passes, alone):
+        assert all(np.array_equal(a, b) for a, b in zip(results(p), want))
+    graph = hip.capture(streams[0], lambda: [step(p, streams[0]) for p in passes])
+    for i in range(4):
+        for p in passes:                                                 # (what the last replay left is gone)
+            for d in (p.out, p.lse, p.mass, p.source, p.id):
+                L.check(lib.pi_memset(d.ptr, 0, d.nbytes, None), "memset")
+            L.check(lib.pi_memcpy_h2d(p.out.ptr, np.full((p.T, p.os), 7.0, np.float32).ctypes.data_as(C.c_void_p), p.out.nbytes, None), "h2d")
+        L.check(lib.pi_device_sync(), "sync")
+        hip.replay(graph, streams[0])
+        L.check(lib.pi_device_sync(), "sync")
+        for p, want in zip(passes, alone):
+            assert all(np.array_equal(a, b) for a, b in zip(results(p), want)), i
+        step(passes[i % 2], None)
+        L.check(lib.pi_device_sync(), "sync")
