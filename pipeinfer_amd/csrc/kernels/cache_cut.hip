@@ -4,12 +4,14 @@
 // there: source[i] = the cell whose rows stand at i afterwards, and no more rows move than have to.
 #include "ops_common.h"
 #include "kernel_timing.h"
+#include "wave_scan.h"
 
 #include <algorithm>
 
 #define CC_THREADS 1024
 #define CC_BINS 2048
-#define CC_WINDOW 32768      /* cells that move, a window of LDS at a time */
+#define CC_KEYS 28672        /* keys in LDS (112 KB); cells that move, as many at a time */
+#define CC_CELLS 131072      /* cells of the bitmap */
 
 // order of the cells: guarded, then by mass (-0 like 0), what is no number last
 static __device__ __forceinline__ uint32_t cc_key(float x, bool guarded) {
@@ -18,11 +20,9 @@ static __device__ __forceinline__ uint32_t cc_key(float x, bool guarded) {
     return guarded ? 0xffffffffu : x != x ? 0u : k;
 }
 
-// inclusive sum over the workgroup's threads before this one in order, and over all (sixteen waves; two barriers)
+// the sum over the workgroup's threads ahead of this one, and over all of them (sixteen waves; two barriers)
 static __device__ __forceinline__ uint32_t cc_before(uint32_t v, uint32_t * waves, int lane, int wave, uint32_t & all) {
-    uint32_t x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const uint32_t y = __shfl_up(x, o, 64); if (lane >= o) x += y; }
+    const uint32_t x = pi_wave_scan(v);
     __syncthreads();
     if (lane == 63) waves[wave] = x;
     __syncthreads();
@@ -32,101 +32,226 @@ static __device__ __forceinline__ uint32_t cc_before(uint32_t v, uint32_t * wave
     return base + x - v;
 }
 
-// One workgroup; a wave owns a run of cells, 64 of them a step.  The boundary's key by its digits of 11, 11 and 10 bits from the counts of what is left.  VPT > 0: the keys of up to 1024 VPT cells stay in registers
-template <int VPT> __global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __restrict__ mass, const uint32_t * __restrict__ guard, int cells, int keep, int32_t * __restrict__ source, const int32_t * __restrict__ abort_w) {
-    if (pi_aborted(abort_w)) return;
-    __shared__ uint32_t bins[CC_BINS];
-    __shared__ int32_t movers[CC_WINDOW];
-    __shared__ uint32_t waves[CC_THREADS / 64], found[3];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, steps = (cells + CC_THREADS - 1) / CC_THREADS;
-    const int64_t first = (int64_t) wave * steps * 64 + lane;
-    uint32_t keys[VPT > 0 ? VPT : 1];
-    auto load = [&](int j) __attribute__((always_inline)) -> uint32_t {
-        const int64_t c = first + (int64_t) j * 64;
-        return c < cells ? cc_key(mass[c], guard && (guard[c >> 5] >> (c & 31) & 1)) : 0u;
+// One workgroup.  The boundary's key: its first 11 bits from the counts of all keys, the rest by digits of 11 and 10 bits of those that share them, listed in LDS (of all keys where the list does not hold them).  What stays is then a bit of
+// a bitmap in LDS, and where a cell goes follows from the bits ahead of it: no pass walks the cells in their order.  Bound by the instructions of one compute unit, a handful per pass and 64 cells: keys of up to CC_KEYS cells stay in LDS,
+// the others' are made again from the masses.
+struct cc_shared {
+    __attribute__((aligned(16))) uint32_t bins[CC_BINS], words[2 * CC_CELLS / 32], waves[CC_THREADS / 64], found[4];
+    __attribute__((aligned(16))) uint32_t keys[CC_KEYS];       // then the cells that move
+};
+__global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __restrict__ mass, const uint32_t * __restrict__ guard, int cells, int keep, int32_t * __restrict__ source, const int32_t * __restrict__ abort_w) {
+    const int gone = pi_abort_peek(abort_w);
+    __shared__ cc_shared L;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    for (int i = tid; i < CC_BINS; i += CC_THREADS) L.bins[i] = 0;
+    if (tid == 0) L.found[3] = 0;
+    if (pi_aborted_together(gone, abort_w)) return;
+    auto count = [&](bool in, uint32_t bin) __attribute__((always_inline)) {
+        const uint32_t b0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) bin);
+        if (__all(in && bin == b0)) { if (lane == 0) atomicAdd(&L.bins[b0], 64u); }              // (equal masses: one address)
+        else if (in) atomicAdd(&L.bins[bin], 1u);
     };
-    if constexpr (VPT > 0) {
+    // the keys, eight cells a thread on their way at a time
+    for (int c0 = 0; c0 < cells; c0 += 8 * CC_THREADS) {
+        float m[8]; uint32_t g[8] = {};
 #pragma unroll
-        for (int j = 0; j < VPT; j++) keys[j] = j < steps ? load(j) : 0u;
+        for (int j = 0; j < 8; j++) m[j] = mass[min(c0 + j * CC_THREADS + tid, cells - 1)];
+        if (guard)
+#pragma unroll
+            for (int j = 0; j < 8; j++) g[j] = guard[min(c0 + j * CC_THREADS + tid, cells - 1) >> 5];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int c = c0 + j * CC_THREADS + tid;
+            if (c - lane >= cells) break;
+            const uint32_t key = cc_key(m[j], g[j] >> (tid & 31) & 1);
+            if (c < CC_KEYS) L.keys[c] = key;
+            count(c < cells, key >> 21);
+        }
     }
-    // f(cell, is one, key) for the wave's cells in their order
+    // f(cell, is one, key) for every CC_THREADS-th cell, whole waves at a time
     auto each = [&](auto && f) __attribute__((always_inline)) {
-        if constexpr (VPT > 0) {
-#pragma unroll
-            for (int j = 0; j < VPT; j++) if (j < steps) { const int64_t c = first + (int64_t) j * 64; f((int) c, c < cells, keys[j]); }
-        } else for (int j = 0; j < steps; j++) { const int64_t c = first + (int64_t) j * 64; f((int) c, c < cells, load(j)); }
+        const int held = min(cells, CC_KEYS);
+        int c = tid;
+        for (; c - lane < held; c += CC_THREADS) f(c, c < cells, L.keys[min(c, CC_KEYS - 1)]);
+        for (; c - lane < cells; c += CC_THREADS) f(c, c < cells, c < cells ? cc_key(mass[c], guard && (guard[c >> 5] >> (c & 31) & 1)) : 0u);
     };
-    uint32_t prefix = 0, left = (uint32_t) keep;               // `left` of the cells whose key begins like `prefix` stay; those above stay, those below do not
+    uint32_t prefix = 0, left = (uint32_t) keep, same = 0;     // of the `same` cells whose key begins like `prefix` `left` stay, the lowest; all above stay, none below
+    // from the top bin down, two to a thread
+    auto border = [&](int width) __attribute__((always_inline)) {
+        __syncthreads();
+        const int top = (1 << width) - 1 - 2 * tid;
+        const uint32_t a = top >= 0 ? L.bins[top] : 0, b = top >= 1 ? L.bins[top - 1] : 0;
+        uint32_t all;
+        const uint32_t before = cc_before(a + b, L.waves, lane, wave, all);
+        if (before < left && before + a + b >= left) {
+            const bool second = before + a < left;
+            L.found[0] = (uint32_t) (second ? top - 1 : top); L.found[1] = left - before - (second ? a : 0); L.found[2] = second ? b : a;
+        }
+        __syncthreads();
+        prefix = prefix << width | L.found[0]; left = L.found[1]; same = L.found[2];
+    };
+    border(11);
+    int shift = 21;
+    const bool listed = same <= 2 * (CC_CELLS / 32);             // (bitmap and sums are not in use yet)
+    uint32_t * const list = L.words, * const bitmap = L.words, * const ahead = L.words + CC_CELLS / 32;
+    const uint32_t in_list = same;
+    if (same != left && listed) {
+        uint32_t mine = 0;                                   // (counted first: no store waits for an atomic)
+        each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { mine += is && key >> 21 == prefix; });
+        if (__any(mine > 0)) {
+            uint32_t at = mine > 0 ? atomicAdd(&L.found[3], mine) : 0;
+            each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { if (is && key >> 21 == prefix) list[at++] = key; });
+        }
+        __syncthreads();
+    }
+    for (int pass = 0; pass < 2 && same != left; pass++) {
+        const int width = 11 - pass, from = shift - width;
+        for (int i = tid; i < CC_BINS; i += CC_THREADS) L.bins[i] = 0;
+        __syncthreads();
+        auto digit = [&](int, bool is, uint32_t key) __attribute__((always_inline)) { count(is && key >> shift == prefix, key >> from & ((1u << width) - 1)); };
+        if (listed) for (uint32_t i = tid; i - lane < in_list; i += CC_THREADS) digit(0, i < in_list, list[min(i, in_list - 1)]);
+        else each(digit);
+        border(width);
+        shift = from;
+    }
+    __syncthreads();
+    // the bitmap of what stays; where not all of the boundary's key do, the first of them
+    const uint32_t bound = prefix << shift;
+    const bool some = same != left;
+    const int words = (cells + 31) / 32;
+    each([&](int c, bool is, uint32_t key) __attribute__((always_inline)) {
+        const unsigned long long who = __ballot(is && key >= bound);
+        if (lane == 0) *(unsigned long long *) (bitmap + c / 32) = who;          // (a step past the end writes zeros)
+        if (some) {
+            const unsigned long long eq = __ballot(is && key >> shift == prefix);
+            if (lane == 0) *(unsigned long long *) (ahead + c / 32) = eq;
+        }
+    });
+    __syncthreads();
+    uint32_t all;
+    if (some) {
+        // of the words' equal ones (in `ahead`) those past the first `left` go
+        for (uint32_t w0 = 0, seen = 0; w0 < (uint32_t) words; w0 += CC_THREADS) {
+            const uint32_t w = w0 + tid;
+            uint32_t eq = w < (uint32_t) words ? ahead[w] : 0, n = seen + cc_before((uint32_t) __popc(eq), L.waves, lane, wave, all);
+            uint32_t go = 0;
+            for (; eq; eq &= eq - 1, n++) if (n >= left) go |= eq & -eq;
+            if (go) bitmap[w] &= ~go;
+            seen += all;
+        }
+        __syncthreads();
+    }
+    // ahead of a word in front of the budget: the places that become free; behind it: the cells that stay (both in the word where it ends)
+    const uint32_t edge = (uint32_t) keep / 32, in_front = (1u << (keep & 31)) - 1;          // of the edge's word
+    uint32_t total = 0, edge_free = 0;
+    for (int part = 0; part < 2; part++) {
+        uint32_t seen = 0;
+        for (uint32_t w0 = part == 0 ? 0 : edge / CC_THREADS * CC_THREADS; w0 < (part == 0 ? edge + 1 : (uint32_t) words); w0 += CC_THREADS) {
+            const uint32_t w = w0 + tid, b = w < (uint32_t) words ? bitmap[w] : 0;
+            const uint32_t mine = part == 0 ? (w < edge ? ~b : w == edge ? ~b & in_front : 0) : (w > edge ? b : w == edge ? b & ~in_front : 0);
+            const uint32_t n = seen + cc_before((uint32_t) __popc(mine), L.waves, lane, wave, all);
+            if (w < (uint32_t) words && (part == 0 ? w < edge : w > edge)) ahead[w] = n;
+            if (part == 0 && w == edge) L.found[0] = n;          // (there the cells that stay begin with none ahead)
+            seen += all;
+        }
+        total = seen;
+        __syncthreads();
+        if (part == 0) edge_free = L.found[0];
+    }
+    for (uint32_t w0 = 0; w0 == 0 || w0 < total; w0 += CC_KEYS) {
+        for (int c = (int) edge * 32 + tid; c < cells; c += CC_THREADS) {
+            const uint32_t w = (uint32_t) c / 32, b = w == edge ? bitmap[w] & ~in_front : bitmap[w];
+            if (!(b >> (c & 31) & 1)) continue;
+            const uint32_t r = (w == edge ? 0 : ahead[w]) + (uint32_t) __popc(b & ((1u << (c & 31)) - 1)) - w0;
+            if (r < CC_KEYS) L.keys[r] = (uint32_t) c;           // (r wraps far above for those of earlier windows)
+        }
+        __syncthreads();
+        for (int c = tid; c < keep; c += CC_THREADS) {
+            const uint32_t w = (uint32_t) c / 32, b = bitmap[w];
+            if (b >> (c & 31) & 1) { if (w0 == 0) source[c] = c; continue; }
+            const uint32_t r = (w == edge ? edge_free : ahead[w]) + (uint32_t) __popc(~b & ((1u << (c & 31)) - 1)) - w0;
+            if (r < CC_KEYS) source[c] = (int32_t) L.keys[r];
+        }
+        __syncthreads();
+    }
+}
+
+// Caches of more cells than the bitmap holds: the same border, then the cells in their order, a wave's run of them 64 a step
+static __device__ __forceinline__ uint32_t cc_rank(unsigned long long who) { return __builtin_amdgcn_mbcnt_hi((uint32_t) (who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) who, 0u)); }
+
+__global__ void __launch_bounds__(CC_THREADS) k_cache_choose_long(const float * __restrict__ mass, const uint32_t * __restrict__ guard, int cells, int keep, int32_t * __restrict__ source, const int32_t * __restrict__ abort_w) {
+    const int gone = pi_abort_peek(abort_w);
+    __shared__ uint32_t bins[CC_BINS], waves[CC_THREADS / 64], found[3], list[CC_KEYS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), steps = (cells + CC_THREADS - 1) / CC_THREADS;
+    const int64_t first = (int64_t) wave * steps * 64;
+    if (pi_aborted_together(gone, abort_w)) return;
+    // f(first cell of the step, is this lane's one, key) for the wave's cells in their order
+    auto each = [&](auto && f) __attribute__((always_inline)) {
+        for (int j = 0; j < steps; j++) {
+            const int64_t c = first + (int64_t) j * 64, mine = c + lane;
+            if (c >= cells) break;
+            f((int) c, mine < cells, mine < cells ? cc_key(mass[mine], guard && (guard[mine >> 5] >> (mine & 31) & 1)) : 0u);
+        }
+    };
+    uint32_t prefix = 0, left = (uint32_t) keep, same = 0, all;
     int shift = 32;
-    for (int pass = 0; pass < 3 && left > 0; pass++) {
+    for (int pass = 0; pass < 3 && same != left; pass++) {
         const int width = pass == 2 ? 10 : 11, from = shift - width;
         for (int i = tid; i < CC_BINS; i += CC_THREADS) bins[i] = 0;
         __syncthreads();
         each([&](int, bool is, uint32_t key) __attribute__((always_inline)) {
             const bool in = is && (pass == 0 || key >> shift == prefix);
-            const uint32_t bin = key >> from & ((1u << width) - 1);
-            const unsigned long long who = __ballot(in);
-            if (who == 0) return;
-            const int lead = __builtin_ctzll(who);
-            const uint32_t b0 = (uint32_t) __builtin_amdgcn_readlane((int) bin, lead);
-            if (__ballot(in && bin == b0) == who) { if (lane == lead) atomicAdd(&bins[b0], (uint32_t) __popcll(who)); }          // (equal masses: one address)
+            const uint32_t bin = key >> from & ((1u << width) - 1), b0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) bin);
+            if (__all(in && bin == b0)) { if (lane == 0) atomicAdd(&bins[b0], 64u); }
             else if (in) atomicAdd(&bins[bin], 1u);
         });
         __syncthreads();
-        // from the top bin down, two to a thread
         const int top = (1 << width) - 1 - 2 * tid;
-        const uint32_t a = top >= 0 ? bins[top] : 0, b = top >= 1 ? bins[top - 1] : 0;
-        uint32_t all, before = cc_before(a + b, waves, lane, wave, all);
+        const uint32_t a = top >= 0 ? bins[top] : 0, b = top >= 1 ? bins[top - 1] : 0, before = cc_before(a + b, waves, lane, wave, all);
         if (a + b > 0 && before < left && before + a + b >= left) {
             const bool second = before + a < left;
             found[0] = (uint32_t) (second ? top - 1 : top); found[1] = left - before - (second ? a : 0); found[2] = second ? b : a;
         }
         __syncthreads();
-        prefix = prefix << width | found[0]; left = found[1]; shift = from;
-        if (found[2] == left) break;                         // all of the bin stay
+        prefix = prefix << width | found[0]; left = found[1]; same = found[2]; shift = from;
     }
-    __syncthreads();
-    // key >> shift > prefix stays; == prefix: the first `left` (all, where the passes ended early)
+    const uint32_t bound = prefix << shift;
     uint32_t equal = 0;
-    auto above = [&](bool is, uint32_t key) __attribute__((always_inline)) { return is && keep > 0 && (shift < 32 ? key >> shift : 0) > prefix; };
-    auto same = [&](bool is, uint32_t key) __attribute__((always_inline)) { return is && keep > 0 && (shift < 32 ? key >> shift : 0) == prefix; };
-    each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { equal += (uint32_t) __popcll(__ballot(same(is, key))); });
-    uint32_t all;
-    const uint32_t equal_before = cc_before(lane == 0 ? equal : 0, waves, lane, wave, all);
-    const uint32_t equal0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) equal_before);
+    each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { equal += (uint32_t) __popcll(__ballot(is && key >> shift == prefix)); });
+    const uint32_t equal0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) cc_before(lane == 0 ? equal : 0, waves, lane, wave, all));
     auto stays = [&](bool is, uint32_t key, uint32_t & seen) __attribute__((always_inline)) {
-        const unsigned long long who = __ballot(same(is, key));
-        const bool mine = same(is, key) && seen + (uint32_t) __popcll(who & ((1ull << lane) - 1)) < left;
+        const bool eq = is && key >> shift == prefix;
+        const unsigned long long who = __ballot(eq);
+        const bool mine = eq ? seen + cc_rank(who) < left : is && key >= bound;
         seen += (uint32_t) __popcll(who);
-        return mine || above(is, key);
+        return mine;
     };
-    uint32_t holes = 0, moves = 0, seen = equal0;
+    uint32_t holes = 0, moves = 0, seen = equal0, total;
     each([&](int c, bool is, uint32_t key) __attribute__((always_inline)) {
         const bool s = stays(is, key, seen);
-        holes += (uint32_t) __popcll(__ballot(is && c < keep && !s)); moves += (uint32_t) __popcll(__ballot(is && c >= keep && s));
+        holes += (uint32_t) __popcll(__ballot(c + lane < keep && !s)); moves += (uint32_t) __popcll(__ballot(c + lane >= keep && s));
     });
-    uint32_t total;
     const uint32_t hole0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) cc_before(lane == 0 ? holes : 0, waves, lane, wave, total));
     const uint32_t move0 = (uint32_t) __builtin_amdgcn_readfirstlane((int) cc_before(lane == 0 ? moves : 0, waves, lane, wave, total));
-    for (uint32_t w = 0; w == 0 || w < total; w += CC_WINDOW) {
+    for (uint32_t w = 0; w == 0 || w < total; w += CC_KEYS) {
         uint32_t at = move0;
         seen = equal0;
         __syncthreads();
         each([&](int c, bool is, uint32_t key) __attribute__((always_inline)) {
-            const bool m = stays(is, key, seen) && c >= keep;
+            const bool m = stays(is, key, seen) && c + lane >= keep;
             const unsigned long long who = __ballot(m);
-            const uint32_t r = at + (uint32_t) __popcll(who & ((1ull << lane) - 1)) - w;
-            if (m && r < CC_WINDOW) movers[r] = c;           // (r wraps far above for those of earlier windows)
+            const uint32_t r = at + cc_rank(who) - w;
+            if (m && r < CC_KEYS) list[r] = (uint32_t) (c + lane);
             at += (uint32_t) __popcll(who);
         });
         __syncthreads();
         at = hole0; seen = equal0;
         each([&](int c, bool is, uint32_t key) __attribute__((always_inline)) {
-            const bool s = stays(is, key, seen), h = is && c < keep && !s;
+            const bool s = stays(is, key, seen), in = c + lane < keep, h = in && !s;
             const unsigned long long who = __ballot(h);
-            const uint32_t r = at + (uint32_t) __popcll(who & ((1ull << lane) - 1)) - w;
-            if (h && r < CC_WINDOW) source[c] = movers[r];
-            if (w == 0 && is && c < keep && s) source[c] = c;
+            const uint32_t r = at + cc_rank(who) - w;
+            if (h && r < CC_KEYS) source[c + lane] = (int32_t) list[r];
+            if (w == 0 && in && s) source[c + lane] = c + lane;
             at += (uint32_t) __popcll(who);
         });
     }
@@ -136,9 +261,8 @@ extern "C" int pi_op_cache_choose(const float * mass, const uint32_t * guard, in
     if (cells < 0 || keep < 0 || keep > cells || cells > 0x7ffff000) { pi_set_error("pi_op_cache_choose: %d of %d cells", keep, cells); return -1; }
     if (keep == 0) return 0;
     if (!mass || !source) { pi_set_error("pi_op_cache_choose: mass or source is NULL"); return -1; }
-#define CC_GO(V) PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, 4.0 * cells + 4.0 * keep, (k_cache_choose<V>), dim3(1), dim3(CC_THREADS), 0, (hipStream_t) stream, mass, guard, cells, keep, source, pi_abort_word())
-    if (cells <= CC_THREADS * 4) CC_GO(4); else if (cells <= CC_THREADS * 16) CC_GO(16); else if (cells <= CC_THREADS * 32) CC_GO(32); else CC_GO(0);
-#undef CC_GO
+    if (cells <= CC_CELLS) PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, 4.0 * cells + 4.0 * keep, k_cache_choose, dim3(1), dim3(CC_THREADS), 0, (hipStream_t) stream, mass, guard, cells, keep, source, pi_abort_word());
+    else PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, 4.0 * cells + 4.0 * keep, k_cache_choose_long, dim3(1), dim3(CC_THREADS), 0, (hipStream_t) stream, mass, guard, cells, keep, source, pi_abort_word());
     PI_CHECK_LAUNCH();
     return 0;
 }
@@ -147,7 +271,7 @@ extern "C" int pi_op_cache_choose(const float * mass, const uint32_t * guard, in
 #define CM_ARRAYS 120        /* of one launch: their addresses are the kernel's arguments */
 struct cm_arrays { uint8_t * at[CM_ARRAYS]; uint64_t bytes[CM_ARRAYS]; };
 
-// row i <- row source[i] of one array's 64 rows a wave: the moves are listed in LDS, and as many lanes as a row has units take one.  Rows come from behind `keep` and go in front of it: nothing is read that another thread writes
+// row i <- row source[i] of one array's `rows` (up to 64) a wave: the moves are listed in LDS, and as many lanes as a row has units take one.  Rows come from behind `keep` and go in front of it: nothing is read that another thread writes
 template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base, uint64_t bytes, const int2 * list, int n, int lane) {
     const uint32_t units = (uint32_t) (bytes / sizeof(T));
     int per = 64;
@@ -167,11 +291,13 @@ template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base
     }
 }
 
-__global__ void __launch_bounds__(256) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int keep, int cells, const int32_t * __restrict__ abort_w) {
+__global__ void __launch_bounds__(256) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int rows, int keep, int cells, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w)) return;
     __shared__ int2 lists[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = (blockIdx.x * 4 + wave) * 64 + lane;
-    const int from = row < keep ? source[row] : -1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row64 = ((int64_t) blockIdx.x * 4 + wave) * rows + lane;
+    const int row = (int) min(row64, (int64_t) keep);
+    const int from = lane < rows && row < keep ? source[row] : -1;
     const bool moves = from >= keep && from < cells;
     const unsigned long long who = __ballot(moves);
     if (moves) lists[wave][__popcll(who & ((1ull << lane) - 1))] = make_int2(row, from);
@@ -194,7 +320,8 @@ extern "C" int pi_op_cache_move(void * const * arrays, const int64_t * row_bytes
         const int n = std::min(CM_ARRAYS, n_arrays - i0);
         double bytes = 0;
         for (int i = 0; i < n; i++) { A.at[i] = (uint8_t *) arrays[i0 + i]; A.bytes[i] = (uint64_t) row_bytes[i0 + i]; bytes += 2.0 * std::min(keep, cells - keep) * row_bytes[i0 + i]; }
-        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) ((keep + 255) / 256), (unsigned) n), dim3(256), 0, (hipStream_t) stream, A, source, keep, cells, pi_abort_word());
+        const int rows = (int64_t) keep * n >= 256 * 1024 ? 64 : 8;           // (few rows: more waves with less to do one after the other)
+        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) ((keep + 4 * rows - 1) / (4 * rows)), (unsigned) n), dim3(256), 0, (hipStream_t) stream, A, source, rows, keep, cells, pi_abort_word());
         PI_CHECK_LAUNCH();
     }
     return 0;

@@ -247,7 +247,7 @@ def chosen(mass, guarded, keep):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("cells", [1, 2, 63, 65, 1000, 4097, 20000, 33000, 100001])
+@pytest.mark.parametrize("cells", [1, 2, 63, 65, 1000, 4097, 20000, 33000, 100001, 131072, 140001])
 def test_choice(cells):
     """masses of every kind: spread, all equal, few different ones, signs, infinities and what is no number; guards, more of them than stay; one cell to all of them"""
     U, lib = gpu()
