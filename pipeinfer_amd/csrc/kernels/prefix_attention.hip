@@ -259,7 +259,7 @@ static __device__ __forceinline__ void px_share(int n, int run, int part, int pa
 }
 
 template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
-    if (pi_aborted(abort_w, 5)) return;
+    if (pi_aborted_together(pi_abort_peek(abort_w), abort_w, 5)) return;
     constexpr int NARROW = 4 * 32 * px_lds<DP>::V + 2 * PX_LIST, MEET = 2 * (DP / 2 + 2) * 256, WIDE_B = WIDE ? 2 * 64 * (px_lds<DP>::K + px_lds<DP>::V) : 0;
     __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? (NARROW > MEET ? NARROW : MEET) : WIDE_B];
     __shared__ int listed[4];
@@ -327,28 +327,54 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
     if (wave == 0) px_leave<DP>(A, S, A.prompt_parts + part, tok, head, in < A.group, g);
 }
 
-// a wave per row: the parts' sums over their joint maximum
-__global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, const int32_t * __restrict__ abort_w) {
+// The parts' sums over their joint maximum.  Four of a row's values to a thread and about every `groups`-th part, the threads of a row meet in LDS: with a wave per row and its parts one after the other the loads' latency was all the
+// time (4096 rows of 17 parts: 24.2 us; 1024 of 17: 20.8)
+#define PX_MERGED 1088
+__global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, int groups, int rows_here, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;
-    const int lane = threadIdx.x & 63;
-    const int64_t rows = (int64_t) A.n_tok * A.heads, r = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    float m = -INFINITY, l = 0.0f, o[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-    for (int p = lane; p < parts; p += 64) { const float2 x = A.parts_ml[p * rows + r]; if (x.y != 0.0f) m = fmaxf(m, x.x); }
-    m = pi_wave_max(m);
-    for (int p = 0; p < parts; p++) {
-        const float2 x = A.parts_ml[p * rows + r];
-        if (x.y == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(x.x - m);
-        l += x.y * f;
+    __shared__ float2 ml[PX_MERGED];
+    __shared__ px_f32x4 sums[256];
+    __shared__ float ls[256];
+    const int tid = threadIdx.x, quads = A.dim / 4, at = tid / quads, d = 4 * (tid % quads), mine = at / groups, grp = at % groups;
+    const int64_t rows = (int64_t) A.n_tok * A.heads, r0 = (int64_t) blockIdx.x * rows_here;
+    const bool on = mine < rows_here && r0 + mine < rows;
+    const float * from = A.parts_o + min(r0 + mine, rows - 1) * A.dim + d;
+    const int64_t step = rows * A.dim;
+    px_f32x4 x[4];
+    auto load = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) { const int d = 64 * i + lane; if (d < A.dim) o[i] += A.parts_o[(p * rows + r) * A.dim + d] * f; }
+        for (int i = 0; i < 4; i++) x[i] = *(const px_f32x4 *) (from + min(p + i * groups, parts - 1) * step);
+    };
+    if (parts > 0) load(grp);
+    for (int i = tid; i < rows_here * parts; i += 256) ml[i] = A.parts_ml[i % parts * rows + min(r0 + i / parts, rows - 1)];
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f;
+    px_f32x4 o = { 0.0f, 0.0f, 0.0f, 0.0f };
+    if (on) {
+        for (int p = 0; p < parts; p++) { const float2 v = ml[mine * parts + p]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
+        for (int p = grp; p < parts; p += 4 * groups) {
+            if (p != grp) load(p);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (p + i * groups >= parts) continue;
+                const float2 v = ml[mine * parts + p + i * groups];
+                if (v.y == 0.0f) continue;                   // (a part without a cell: its outputs are not there)
+                const float f = __builtin_amdgcn_exp2f(v.x - m);
+                l += v.y * f; o += x[i] * f;
+            }
+        }
     }
+    if (groups > 1) {
+        sums[tid] = o; ls[tid] = l;
+        __syncthreads();
+        if (grp != 0 || !on) return;
+        for (int i = 1; i < groups; i++) { o += sums[tid + i * quads]; l += ls[tid + i * quads]; }
+    }
+    if (!on) return;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    float * to = A.out + r / A.heads * A.out_stride + r % A.heads * A.dim;
-#pragma unroll
-    for (int i = 0; i < 4; i++) { const int d = 64 * i + lane; if (d < A.dim) to[d] = o[i] * f; }
-    if (lane == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+    const int64_t r = r0 + mine;
+    *(px_f32x4 *) (A.out + r / A.heads * A.out_stride + r % A.heads * A.dim + d) = o * f;
+    if (d == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
 }
 
 // ---- how the work is cut ---------------------------------------------------------------------------------------------------------------------------------------------------------------
@@ -394,8 +420,12 @@ template <int DP> static int px_launch(const px_args & A, hipStream_t s) {
         PI_CHECK_LAUNCH();
     }
     if (parts != 1) {
-        const unsigned grid = (unsigned) (((int64_t) A.n_tok * A.heads + 3) / 4);
-        PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 4.0 * A.n_tok * A.heads * ((double) parts * (A.dim + 2) + A.dim), k_prefix_merge, dim3(grid), dim3(256), 0, s, A, parts, pi_abort_word());
+        const int at_once = 256 / (A.dim / 4);
+        int groups = 1;
+        while (groups * 4 < parts && groups * 2 <= at_once) groups *= 2;
+        const int here = at_once / groups;
+        const int64_t grid = ((int64_t) A.n_tok * A.heads + here - 1) / here;
+        PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 4.0 * A.n_tok * A.heads * ((double) parts * (A.dim + 2) + A.dim), k_prefix_merge, dim3((unsigned) grid), dim3(256), 0, s, A, parts, groups, here, pi_abort_word());
         PI_CHECK_LAUNCH();
     }
     return 0;
@@ -535,6 +565,7 @@ __global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, 
     const int64_t cell = (int64_t) blockIdx.x * 256 + threadIdx.x;
     if (cell >= n_kv) return;
     float x = 0.0f;
+#pragma unroll 16
     for (int p = 0; p < parts; p++) x += A.parts[(int64_t) p * A.n_kv + cell];
     A.mass[cell] = A.decay == 0.0f ? x : A.decay * A.mass[cell] + x;
 }
@@ -542,7 +573,11 @@ __global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, 
 static void pm_plan(pm_args & A) {
     const int rows = A.n_tok * A.group;
     A.cell_blocks = (A.n_kv + 255) / 256;
-    A.row_parts = (int) std::max<int64_t>(1, std::min<int64_t>(2 * pi_cu_count() / std::max<int64_t>(1, (int64_t) A.cell_blocks * A.kv), (rows + 63) / 64));
+    // as many parts of the rows as leave the fewest workgroup rounds of the chip's two per compute unit idle, at most one for every 64 rows
+    const int64_t units = (int64_t) A.cell_blocks * A.kv, slots = 2 * pi_cu_count();
+    A.row_parts = 1;
+    double least = 1e30;
+    for (int p = 1; p <= 16 && p <= (rows + 63) / 64; p++) { const double t = (double) ((units * p + slots - 1) / slots) * (1.0 / p + 0.03); if (t < least * 0.98) { least = t; A.row_parts = p; } }
 }
 static size_t pm_floats(const pm_args & A) { const size_t parts = (size_t) A.kv * A.row_parts; return parts > 1 ? parts * A.n_kv : 0; }
 
