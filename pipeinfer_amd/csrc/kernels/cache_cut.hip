@@ -271,7 +271,7 @@ extern "C" int pi_op_cache_choose(const float * mass, const uint32_t * guard, in
 #define CM_ARRAYS 120        /* of one launch: their addresses are the kernel's arguments */
 struct cm_arrays { uint8_t * at[CM_ARRAYS]; uint64_t bytes[CM_ARRAYS]; };
 
-// row i <- row source[i] of one array's `rows` (up to 64) a wave: the moves are listed in LDS, and as many lanes as a row has units take one.  Rows come from behind `keep` and go in front of it: nothing is read that another thread writes
+// row i <- row source[i] of one array's 64 rows a wave: the moves are listed in LDS, and as many lanes as a row has units take one.  Rows come from behind `keep` and go in front of it: nothing is read that another thread writes
 template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base, uint64_t bytes, const int2 * list, int n, int lane) {
     const uint32_t units = (uint32_t) (bytes / sizeof(T));
     int per = 64;
@@ -291,19 +291,20 @@ template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base
     }
 }
 
-__global__ void __launch_bounds__(256) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int rows, int keep, int cells, const int32_t * __restrict__ abort_w) {
+// An array's address stands in the kernel's arguments, in host memory: that read is most of a short move, 3 us for one workgroup's, and the reads of all of them queue (45 arrays of 1000 rows, 331 moving: 1440 workgroups of 256 threads 18 us,
+// 45 of 1024 9).  So a workgroup takes 1024 rows of one array
+__global__ void __launch_bounds__(1024) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int blocks, int keep, int cells, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w)) return;
-    __shared__ int2 lists[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row64 = ((int64_t) blockIdx.x * 4 + wave) * rows + lane;
-    const int row = (int) min(row64, (int64_t) keep);
-    const int from = lane < rows && row < keep ? source[row] : -1;
+    __shared__ int2 lists[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, array = (int) blockIdx.x / blocks, block = (int) blockIdx.x % blocks;
+    uint8_t * base = A.at[array];
+    const uint64_t bytes = A.bytes[array];
+    const int64_t row64 = ((int64_t) block * 16 + wave) * 64 + lane;
+    const int row = (int) min(row64, (int64_t) keep), from = row < keep ? source[row] : -1;
     const bool moves = from >= keep && from < cells;
     const unsigned long long who = __ballot(moves);
     if (moves) lists[wave][__popcll(who & ((1ull << lane) - 1))] = make_int2(row, from);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    uint8_t * base = A.at[blockIdx.y];
-    const uint64_t bytes = A.bytes[blockIdx.y];
     const int n = __popcll(who);
     if ((((uintptr_t) base | bytes) & 15) == 0) cm_rows<uint4>(base, bytes, lists[wave], n, lane);
     else if ((((uintptr_t) base | bytes) & 3) == 0) cm_rows<uint32_t>(base, bytes, lists[wave], n, lane);
@@ -320,8 +321,9 @@ extern "C" int pi_op_cache_move(void * const * arrays, const int64_t * row_bytes
         const int n = std::min(CM_ARRAYS, n_arrays - i0);
         double bytes = 0;
         for (int i = 0; i < n; i++) { A.at[i] = (uint8_t *) arrays[i0 + i]; A.bytes[i] = (uint64_t) row_bytes[i0 + i]; bytes += 2.0 * std::min(keep, cells - keep) * row_bytes[i0 + i]; }
-        const int rows = (int64_t) keep * n >= 256 * 1024 ? 64 : 8;           // (few rows: more waves with less to do one after the other)
-        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) ((keep + 4 * rows - 1) / (4 * rows)), (unsigned) n), dim3(256), 0, (hipStream_t) stream, A, source, rows, keep, cells, pi_abort_word());
+        const int blocks = (keep + 1023) / 1024;
+        if ((int64_t) n * blocks > 0x7fffffff) { pi_set_error("pi_op_cache_move: %d rows of %d arrays", keep, n); return -1; }
+        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) (n * blocks)), dim3(1024), 0, (hipStream_t) stream, A, source, blocks, keep, cells, pi_abort_word());
         PI_CHECK_LAUNCH();
     }
     return 0;

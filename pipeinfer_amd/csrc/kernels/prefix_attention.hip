@@ -29,8 +29,8 @@ static __device__ __forceinline__ int px_cell(int i, int g) { return 8 * (i >> 2
 // Bytes between rows in LDS.  Keys: an odd number of 16 bytes, so that the rows of a read of 16 bytes a lane lie apart.  Values: a transposing read takes 64 bytes of four rows for 32 lanes: 64 or 192 modulo 256
 template <int DP> struct px_lds { static constexpr int K = 2 * DP + 16, V = (DP / 32) % 2 ? 2 * DP : 2 * DP + 64; };
 
-#define PX_LIFT 6.0f        /* weights are held times 2^6, 2^14 where the maximum lags: fp16's smallest steps are then 2^-30 of the largest weight */
-#define PX_LAG 8.0f         /* the maximum that weights are relative to follows when it has grown by 2^8 */
+#define PX_LIFT 6.0f        /* weights are held times 2^6 or more: fp16's smallest steps are then 2^-30 of the largest weight */
+#define PX_MOST 32768.0f    /* the maximum that weights are relative to follows when those of a lane's sixteen cells exceed this: fp16 holds them until then */
 #define PX_LIST 8192        /* cells of 256 words of a mask */
 
 // 32 queries of one key head, a column of the tile per lane, lanes l and l + 32 the same: their sums so far.  Of acc the outputs 32 j + px_cell(i, g); m in powers of two, l of the lane's own cells
@@ -50,24 +50,32 @@ template <int DP, class K, class V> static __device__ __forceinline__ void px_ti
 #pragma unroll
         for (int i = 0; i < 16; i++) if (px_cell(i, g) >= live) s[i] = -INFINITY;
     }
-    float top = s[0];
+    float p[16], l;
+    auto weigh = [&]() __attribute__((always_inline)) {
+        const float lift = PX_LIFT - (S.m == -INFINITY ? 0.0f : S.m);
 #pragma unroll
-    for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
-    top = fmaxf(top, s[15]);
-    top = fmaxf(top, pi_partner<32>(top)) * c;
-    if (__any(top > S.m + PX_LAG)) {
+        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, lift));
+        l = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) + (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+    };
+    weigh();
+    // (the maximum is looked for where a lane's weights say that it has grown, or that there was none: it costs a dozen instructions a tile)
+    if (__any(l > PX_MOST || S.m == -INFINITY)) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+        top = fmaxf(top, s[15]);
+        top = fmaxf(top, pi_partner<32>(top)) * c;
         const float m = fmaxf(S.m, top), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);
         S.m = m; S.l *= f;
 #pragma unroll
         for (int j = 0; j < DP / 32; j++)
 #pragma unroll
             for (int i = 0; i < 16; i++) S.acc[j][i] *= f;
+        weigh();
     }
-    const float lift = PX_LIFT - (S.m == -INFINITY ? 0.0f : S.m);
-    float p[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, lift));
-    S.l += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) + (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+    S.l += l;
+    float minus = -1.0f;
+    asm("" : "+v"(minus));                                   // (unknown to the compiler: a - h would be a conversion and a subtraction, fma takes the fp16 as it is)
     px_u32x4 hi[2], lo[2];
 #pragma unroll
     for (int z = 0; z < 2; z++)
@@ -76,7 +84,7 @@ template <int DP, class K, class V> static __device__ __forceinline__ void px_ti
             const float a = p[8 * z + 2 * e], b = p[8 * z + 2 * e + 1];
             const px_half2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
             hi[z][e] = __builtin_bit_cast(uint32_t, h);
-            lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], -1.0f, a), fmaf((float) h[1], -1.0f, b)));
+            lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], minus, a), fmaf((float) h[1], minus, b)));
         }
 #pragma unroll
     for (int j = 0; j < DP / 32; j++)
@@ -151,13 +159,16 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
     px_sums<DP> S;
     px_start(S);
     const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
+    // (a chunk past the head's end reads its first: the queries are zero there, and such outputs do not leave)
     auto load = [&](int c) __attribute__((always_inline)) {
+        const uint16_t * kc = k + (int64_t) c * A.row, * vc = v + (int64_t) c * A.row;
+        const int last = c1 - 1 - c;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int x = i * 256 + tid, d = x % CH * 8;
-            const int64_t o = (int64_t) min(c + x / CH, c1 - 1) * A.row + d;
-            kr[i] = d < A.dim ? *(const px_u32x4 *) (k + o) : px_u32x4{ 0, 0, 0, 0 };
-            vr[i] = d < A.dim ? *(const px_u32x4 *) (v + o) : px_u32x4{ 0, 0, 0, 0 };
+            const uint32_t o = (uint32_t) (last >= 63 ? x / CH : min(x / CH, last)) * (uint32_t) A.row + (uint32_t) (d < A.dim ? d : 0);
+            kr[i] = *(const px_u32x4 *) (kc + o);
+            vr[i] = *(const px_u32x4 *) (vc + o);
         }
     };
     auto store = [&](uint8_t * to) __attribute__((always_inline)) {
@@ -196,13 +207,13 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
     const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
     px_u32x4 kr[N], vr[N];
     auto load = [&](int at) __attribute__((always_inline)) {
-        const int64_t o = (int64_t) cell_of(min(at + n, count - 1)) * A.row;
+        const uint16_t * kc = k + (int64_t) cell_of(min(at + n, count - 1)) * A.row;
 #pragma unroll
-        for (int i = 0; i < N; i++) kr[i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (k + o + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+        for (int i = 0; i < N; i++) kr[i] = *(const px_u32x4 *) (kc + (16 * i + 8 * g < A.dim ? 16 * i + 8 * g : 0));
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int x = i * 64 + lane, d = x % CH * 8;
-            vr[i] = d < A.dim ? *(const px_u32x4 *) (v + (int64_t) cell_of(min(at + x / CH, count - 1)) * A.row + d) : px_u32x4{ 0, 0, 0, 0 };
+            vr[i] = *(const px_u32x4 *) (v + (int64_t) cell_of(min(at + x / CH, count - 1)) * A.row + (d < A.dim ? d : 0));
         }
     };
     if (32 * wave >= count) return;
@@ -392,6 +403,7 @@ static void px_plan(px_args & A) {
 
 static int px_sizes(const char * what, int dim, int heads, int kv, int n_tok, int prompt, int n_kv) {
     if (heads < 1 || kv < 1 || heads % kv || dim < 8 || dim > 256 || dim % 8) { pi_set_error("%s: %d query heads over %d key / value heads of %d values (whole groups; 8 .. 256 values in steps of 8)", what, heads, kv, dim); return -1; }
+    if ((int64_t) kv * dim > 1 << 22) { pi_set_error("%s: cells of %d x %d values", what, kv, dim); return -1; }
     if (n_tok < 0 || prompt < 0 || prompt > n_kv || n_kv > 0x7fffff00 || (int64_t) n_tok * heads > 0x3fffffff) { pi_set_error("%s: %d tokens of %d heads, %d of %d cells shared", what, n_tok, heads, prompt, n_kv); return -1; }
     return 0;
 }
@@ -491,8 +503,9 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
     auto load = [&](int r) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            // (past the head's end the keys are zero; what is multiplied there is the head's first values)
             const int x = i * 256 + tid, d = x % CH * 8, m = min(r + x / CH, r1 - 1);
-            qr[i] = d < A.dim ? *(const px_u32x4 *) (A.q + (int64_t) (m / A.group) * A.q_stride + (int64_t) (kvh * A.group + m % A.group) * A.dim + d) : px_u32x4{ 0, 0, 0, 0 };
+            qr[i] = *(const px_u32x4 *) (A.q + (int64_t) (m / A.group) * A.q_stride + (int64_t) (kvh * A.group + m % A.group) * A.dim + (d < A.dim ? d : 0));
         }
         if (tid < 64) {
             const int m = min(r + tid, r1 - 1);
@@ -513,36 +526,40 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         __syncthreads();
         const bool more = r + 64 < r1;
         if (more) load(r + 64);
+        // (cells that every row sees have no test: half of the vector instructions are exponentials' then)
+        auto rows = [&](auto with_mask) __attribute__((always_inline)) {
 #pragma unroll
-        for (int v = 0; v < 2; v++) {
-            if (r + 32 * v >= r1) continue;
-            const uint8_t * qt = lds + cur * STAGE + (32 * v + n) * KS + 16 * g;
-            const float l = lse[cur][32 * v + n];
+            for (int v = 0; v < 2; v++) {
+                if (r + 32 * v >= r1) continue;
+                const uint8_t * qt = lds + cur * STAGE + (32 * v + n) * KS + 16 * g;
+                const float l = lse[cur][32 * v + n];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int base = mine + 32 * u;
-                uint32_t bits = ~0u;
-                if (masked) {
-                    bits = 0;
-                    if (base < n_kv) {
-                        if (base + 32 > prompt) bits = A.mask[(int64_t) (min(r + 32 * v + n, r1 - 1) / A.group) * words + base / 32];
-                        if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
-                        if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
+                for (int u = 0; u < 2; u++) {
+                    const int base = mine + 32 * u;
+                    uint32_t bits = ~0u;
+                    if constexpr (with_mask) {
+                        bits = 0;
+                        if (base < n_kv) {
+                            if (base + 32 > prompt) bits = A.mask[(int64_t) (min(r + 32 * v + n, r1 - 1) / A.group) * words + base / 32];
+                            if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
+                            if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
+                        }
+                        if (!__any(bits != 0)) continue;
                     }
-                    if (!__any(bits != 0)) continue;
+                    px_f32x16 s = px_zero();
+#pragma unroll
+                    for (int i = 0; i < DP / 16; i++) s = px_mfma(key[u][i], *(const px_u32x4 *) (qt + 32 * i), s);
+                    if constexpr (with_mask) {
+                        bits >>= 4 * g;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[u][i] += __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -l));
                 }
-                px_f32x16 s = px_zero();
-#pragma unroll
-                for (int i = 0; i < DP / 16; i++) s = px_mfma(key[u][i], *(const px_u32x4 *) (qt + 32 * i), s);
-                if (masked) {
-                    bits >>= 4 * g;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) if (!(bits >> (8 * (i >> 2) + (i & 3)) & 1)) s[i] = -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) sum[u][i] += __builtin_amdgcn_exp2f(fmaf(s[i], A.c, -l));
             }
-        }
+        };
+        if (masked) rows(std::true_type{}); else rows(std::false_type{});
         if (more) store(cur ^ 1);
     }
 #pragma unroll
