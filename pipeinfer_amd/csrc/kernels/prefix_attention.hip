@@ -9,6 +9,7 @@
 // Sums and statistics are fp32.  Products are fp16 x fp16 (exact in fp32); a weight is two fp16 values, what the first leaves and the second again cuts off (22 bits; one alone, 11 bits, is 1.4e-4 off over 32000 cells).
 #include "ops_common.h"
 #include "kernel_timing.h"
+#include "wave_scan.h"
 
 #include <algorithm>
 #include <cmath>
@@ -31,7 +32,7 @@ template <int DP> struct px_lds { static constexpr int K = 2 * DP + 16, V = (DP 
 
 #define PX_LIFT 6.0f        /* weights are held times 2^6 or more: fp16's smallest steps are then 2^-30 of the largest weight */
 #define PX_MOST 32768.0f    /* the maximum that weights are relative to follows when those of a lane's sixteen cells exceed this: fp16 holds them until then */
-#define PX_LIST 8192        /* cells of 256 words of a mask */
+#define PX_LIST 2048        /* cells of 64 words of a mask, a wave's */
 
 // 32 queries of one key head, a column of the tile per lane, lanes l and l + 32 the same: their sums so far.  Of acc the outputs 32 j + px_cell(i, g); m in powers of two, l of the lane's own cells
 template <int DP> struct px_sums { px_f32x16 acc[DP / 32]; float m, l; };
@@ -105,13 +106,24 @@ template <int STRIDE> static __device__ __forceinline__ px_u32x4 px_value(const 
     return px_u32x4{ a[0], a[1], b[0], b[1] };
 }
 
+// n / d for n < 2^31 (a division by what only the arguments know is thirty instructions, and a kernel that runs for a few us waits for every line of code that it has not run yet: 80 clocks for 64 bytes)
+struct px_div { uint32_t mul, shift; };
+static px_div px_divide_by(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    return { (uint32_t) (((1ull << (31 + s)) + d - 1) / d), 31 + s };
+}
+static __device__ __forceinline__ uint32_t px_quotient(uint32_t n, px_div d) { return (uint32_t) (((uint64_t) n * d.mul) >> d.shift); }
+
 struct px_args {
     const uint16_t * q; int64_t q_stride;
     const uint16_t * k, * v; int64_t row;                    // a cell's values: all key heads
     const uint32_t * mask; const int32_t * dyn;
     float c;
     int dim, heads, kv, group, n_tok, prompt, n_kv;
-    int rows_of, row_blocks, prompt_parts, own_blocks, own_parts;   // rows of a workgroup; of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
+    int row_blocks, prompt_parts, own_blocks, own_parts;     // of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
+    px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts;
+    int prompt_share, own_share;                             // cells, words of the mask of a part where the sizes are the arguments'
     float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
     float * out; int64_t out_stride; float * lse;
 };
@@ -153,7 +165,7 @@ template <int DP> static __device__ __forceinline__ void px_queries(const px_arg
 template <int DP> static __device__ __forceinline__ void px_wide(const px_args & A, uint8_t * lds, int kvh, int block, int part, int c0, int c1) {
     constexpr int KS = px_lds<DP>::K, VS = px_lds<DP>::V, STAGE = 64 * (KS + VS), N = DP / 32, CH = DP / 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5, rows = A.n_tok * A.group;
-    const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = at / A.group, head = kvh * A.group + at % A.group;
+    const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group), head = kvh * A.group + at - tok * A.group;
     px_u32x4 q[DP / 16], kr[N], vr[N];
     px_queries<DP>(A, q, tok, head, g);
     px_sums<DP> S;
@@ -199,9 +211,9 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
     px_leave<DP>(A, S, part, tok, head, row < rows, g);
 }
 
-// Few rows, 32 of them to a workgroup: its waves walk every fourth run of 32 cells each and meet at the end.  `count` cells, the i-th of them at cell_of(i); sums go on in S.  Keys come as operands, values to a part of LDS that is the wave's
+// Few rows, 32 of them: a wave walks the runs of 32 cells first, first + step, .. of `count`, the i-th at cell_of(i); sums go on in S.  Keys come as operands, values to a part of LDS that is the wave's
 // own, so that no wave waits for another; the next run's are on their way meanwhile
-template <int DP, class C> static __device__ __forceinline__ void px_walk(const px_args & A, px_sums<DP> & S, const px_u32x4 (&q)[DP / 16], uint8_t * mine, int kvh, int wave, int lane, int count, C && cell_of) {
+template <int DP, class C> static __device__ __forceinline__ void px_walk(const px_args & A, px_sums<DP> & S, const px_u32x4 (&q)[DP / 16], uint8_t * mine, int kvh, int first, int step, int lane, int count, C && cell_of) {
     constexpr int VS = px_lds<DP>::V, CH = DP / 8, N = DP / 16;
     const int n = lane & 31, g = lane >> 5;
     const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
@@ -216,9 +228,9 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
             vr[i] = *(const px_u32x4 *) (v + (int64_t) cell_of(min(at + x / CH, count - 1)) * A.row + (d < A.dim ? d : 0));
         }
     };
-    if (32 * wave >= count) return;
-    load(32 * wave);
-    for (int at = 32 * wave; at < count; at += 128) {
+    if (first >= count) return;
+    load(first);
+    for (int at = first; at < count; at += step) {
         px_u32x4 kc[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -227,115 +239,111 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
             *(px_u32x4 *) (mine + x / CH * VS + x % CH * 16) = vr[i];
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        if (at + 128 < count) load(at + 128);
+        if (at + step < count) load(at + step);
         const uint8_t * vt = mine + px_value_at(lane, VS);
         px_tile<DP>(S, q, A.c, count - at, g, [&](int i) __attribute__((always_inline)) { return kc[i]; }, [&](int j, int z) __attribute__((always_inline)) { return px_value<VS>(vt, j, z); });
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
-// the sums of the four waves into the first one's, two at a time; lds: 2 * (DP + 2) * 256 bytes, no wave in its own part any more
-template <int DP> static __device__ __forceinline__ void px_meet(px_sums<DP> & S, uint8_t * lds, int wave, int lane) {
-    S.l += pi_partner<32>(S.l);
-    float * at = (float *) lds + (wave & 1) * (DP / 2 + 2) * 64 + lane;
+// the sums of the four waves, of the same rows, put together in LDS by all of them and left as px_leave does; lds: 4 * DP * 128 bytes and 1 KB behind, no wave in its own part any more
+template <int DP> static __device__ __forceinline__ void px_meet(const px_args & A, px_sums<DP> & S, uint8_t * lds, int wave, int lane, int part, int tok, int head, bool mine) {
+    const int n = lane & 31, g = lane >> 5;
+    float2 * const ml = (float2 *) (lds + 4 * DP * 128);
+    const float own = S.l + pi_partner<32>(S.l);
+    __syncthreads();
+    if (g == 0) ml[wave * 32 + n] = make_float2(S.m, own);
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            float * to = (float *) lds + (wave - half) * (DP / 2 + 2) * 64 + lane;
+    for (int w = 0; w < 4; w++) { const float2 x = ml[w * 32 + n]; if (x.y != 0.0f) m = fmaxf(m, x.x); }
 #pragma unroll
-            for (int j = 0; j < DP / 32; j++)
+    for (int w = 0; w < 4; w++) { const float2 x = ml[w * 32 + n]; if (x.y != 0.0f) l += x.y * __builtin_amdgcn_exp2f(x.x - m); }
+    const bool last = A.prompt_parts + A.own_parts == 1;
+    const float f = own == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(S.m - m) * (last ? 1.0f / l : 1.0f);
+    px_f32x4 * const at = (px_f32x4 *) lds;                  // [4 j + i / 4][wave][lane]
 #pragma unroll
-                for (int i = 0; i < 16; i++) to[(16 * j + i) * 64] = S.acc[j][i];
-            to[DP / 2 * 64] = S.m; to[(DP / 2 + 1) * 64] = S.l;
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float om = at[DP / 2 * 64], ol = at[(DP / 2 + 1) * 64], m = fmaxf(S.m, om);
-            const float a = S.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(S.m - m), b = om == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(om - m);
-            S.m = m; S.l = S.l * a + ol * b;
+    for (int j = 0; j < DP / 32; j++)
 #pragma unroll
-            for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) S.acc[j][i] = S.acc[j][i] * a + at[(16 * j + i) * 64] * b;
-        }
+        for (int i = 0; i < 16; i += 4) at[((4 * j + i / 4) * 4 + wave) * 64 + lane] = px_f32x4{ S.acc[j][i] * f, S.acc[j][i + 1] * f, S.acc[j][i + 2] * f, S.acc[j][i + 3] * f };
+    __syncthreads();
+    const int64_t r = (int64_t) tok * A.heads + head, to = (int64_t) part * A.n_tok * A.heads + r;
+    if (wave == 0 && g == 0 && mine) {
+        if (!last) A.parts_ml[to] = make_float2(m, l);
+        else if (A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
     }
-    S.l *= 0.5f;                                             // (px_leave adds the halves)
+    if (!mine || (l == 0.0f && !last)) return;               // (k_prefix_merge leaves such a part out)
+    float * o = last ? A.out + (int64_t) tok * A.out_stride + (int64_t) head * A.dim : A.parts_o + to * A.dim;
+#pragma unroll
+    for (int k = 0; k < DP / 32; k++) {
+        const int i = 4 * k + wave, d = 8 * i + 4 * g;
+        const px_f32x4 a = at[(i * 4) * 64 + lane], b = at[(i * 4 + 1) * 64 + lane], c = at[(i * 4 + 2) * 64 + lane], e = at[(i * 4 + 3) * 64 + lane];
+        if (d < A.dim) *(px_f32x4 *) (o + d) = (a + b) + (c + e);
+    }
 }
 
-// part `part` of `parts` of n things in runs of `run`
-static __device__ __forceinline__ void px_share(int n, int run, int part, int parts, int & from, int & to) {
-    const int64_t runs = (n + run - 1) / run;
-    from = (int) min((int64_t) n, runs * part / parts * run); to = (int) min((int64_t) n, runs * (part + 1) / parts * run);
-}
+// part `part` of n things in shares of `share`
+static __device__ __forceinline__ void px_share(int n, int share, int part, int & from, int & to) { from = (int) min((int64_t) n, (int64_t) part * share); to = (int) min((int64_t) n, (int64_t) from + share); }
+// a share of n things in whole runs of `run`, so that `parts` of them are all
+static __host__ __device__ __forceinline__ int px_share_of(int n, int run, int parts) { const uint32_t runs = ((uint32_t) n + run - 1) / run; return (int) ((runs + parts - 1) / parts) * run; }
 
 template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
-    if (pi_aborted_together(pi_abort_peek(abort_w), abort_w, 5)) return;
-    constexpr int NARROW = 4 * 32 * px_lds<DP>::V + 2 * PX_LIST, MEET = 2 * (DP / 2 + 2) * 256, WIDE_B = WIDE ? 2 * 64 * (px_lds<DP>::K + px_lds<DP>::V) : 0;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? (NARROW > MEET ? NARROW : MEET) : WIDE_B];
-    __shared__ int listed[4];
+    if (pi_aborted(abort_w, 5)) return;                      // (what a wave takes from LDS as an index, it has put there itself)
+    constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 2 * 64 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? NARROW : WIDE_B];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
     const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv);
-    const int pairs = A.kv * A.prompt_parts, prompt_blocks = pairs * A.row_blocks;
+    const uint32_t pairs = (uint32_t) A.kv * A.prompt_parts, prompt_blocks = pairs * A.row_blocks;
     px_u32x4 q[DP / 16];
     px_sums<DP> S;
     uint8_t * mine = lds + wave * 32 * px_lds<DP>::V;
-    if ((int) blockIdx.x < prompt_blocks) {
+    if (blockIdx.x < prompt_blocks) {
         // the blocks of rows that read the same keys follow each other on one XCD (a workgroup's is its number modulo 8)
-        int b = blockIdx.x, pair = b / A.row_blocks, block = b % A.row_blocks;
-        if (pairs % 8 == 0) { pair = b / (8 * A.row_blocks) * 8 + b % 8; block = b / 8 % A.row_blocks; }
-        const int kvh = pair % A.kv, part = pair / A.kv;
+        const uint32_t b = blockIdx.x, eights = pairs % 8 == 0, of = eights ? b >> 3 : b, by = px_quotient(of, A.by_row_blocks), block = of - by * A.row_blocks, pair = eights ? by * 8 + (b & 7) : by;
+        const uint32_t part = px_quotient(pair, A.by_kv), kvh = pair - part * A.kv;
         int c0, c1;
-        px_share(prompt, WIDE ? 64 : 32, part, A.prompt_parts, c0, c1);
+        px_share(prompt, A.dyn ? px_share_of(prompt, WIDE ? 64 : 32, A.prompt_parts) : A.prompt_share, (int) part, c0, c1);
+        const int rows = A.n_tok * A.group;
         if constexpr (WIDE) {
             if (c0 >= c1) {                                  // (fewer cells than there may be)
                 px_start(S);
-                const int row = block * 128 + wave * 32 + n, rows = A.n_tok * A.group, at = min(row, rows - 1);
-                px_leave<DP>(A, S, part, at / A.group, kvh * A.group + at % A.group, row < rows, g);
-            } else px_wide<DP>(A, lds, kvh, block, part, c0, c1);
+                const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group);
+                px_leave<DP>(A, S, (int) part, tok, (int) kvh * A.group + at - tok * A.group, row < rows, g);
+            } else px_wide<DP>(A, lds, (int) kvh, (int) block, (int) part, c0, c1);
         } else {
-            const int rows = A.n_tok * A.group, row = block * 32 + n, at = min(row, rows - 1), tok = at / A.group, head = kvh * A.group + at % A.group;
+            const int row = block * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group), head = (int) kvh * A.group + at - tok * A.group;
             px_queries<DP>(A, q, tok, head, g);
             px_start(S);
-            px_walk<DP>(A, S, q, mine, kvh, wave, lane, c1 - c0, [&](int i) __attribute__((always_inline)) { return c0 + i; });
-            px_meet<DP>(S, lds, wave, lane);
-            if (wave == 0) px_leave<DP>(A, S, part, tok, head, row < rows, g);
+            px_walk<DP>(A, S, q, mine, (int) kvh, 32 * wave, 128, lane, c1 - c0, [&](int i) __attribute__((always_inline)) { return c0 + i; });
+            px_meet<DP>(A, S, lds, wave, lane, (int) part, tok, head, row < rows);
         }
         return;
     }
-    // a token's own cells: 32 of the query heads of one key head
-    int b = blockIdx.x - prompt_blocks;
-    const int kvh = b % A.kv, block = b / A.kv % A.own_blocks, part = b / (A.kv * A.own_blocks) % A.own_parts, tok = b / (A.kv * A.own_blocks * A.own_parts);
-    const int in = block * 32 + n, head = kvh * A.group + min(in, A.group - 1), words = (A.n_kv + 31) / 32, w0 = prompt / 32, w_all = (n_kv + 31) / 32 - w0;
-    uint16_t * list = (uint16_t *) (lds + 4 * 32 * px_lds<DP>::V);
-    px_queries<DP>(A, q, tok, head, g);
-    px_start(S);
+    // a token's own cells: a wave takes 32 of the query heads of one key head, and 64 words of the mask at a time
+    const uint32_t unit = (blockIdx.x - prompt_blocks) * 4 + __builtin_amdgcn_readfirstlane(wave);
+    const uint32_t a = px_quotient(unit, A.by_kv), kvh = unit - a * A.kv, c = px_quotient(a, A.by_own_blocks), block = a - c * A.own_blocks, tok = px_quotient(c, A.by_own_parts), part = c - tok * A.own_parts;
+    if (tok >= (uint32_t) A.n_tok) return;
+    const int in = (int) block * 32 + n, head = (int) kvh * A.group + min(in, A.group - 1), words = (A.n_kv + 31) / 32, w0 = prompt / 32, w_all = max(0, (n_kv + 31) / 32 - w0);
+    uint16_t * list = (uint16_t *) (lds + 4 * 32 * px_lds<DP>::V) + wave * PX_LIST;
     int from, to;
-    px_share(max(0, w_all), 8, part, A.own_parts, from, to);
-    for (int w = from; w < to; w += 256) {
-        uint32_t bits = 0;
-        if (w + tid < to) {
-            const int at = w0 + w + tid;
-            bits = A.mask[(int64_t) tok * words + at];
-            if (32 * at < prompt) bits &= ~0u << (prompt - 32 * at);            // (prompt - 32 * at < 32: at >= prompt / 32)
-            if (n_kv - 32 * at < 32) bits &= (1u << (n_kv - 32 * at)) - 1;
-        }
-        int before = __popc(bits);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(before, o, 64); if (lane >= o) before += x; }
-        __syncthreads();                                     // (the last round's list has been read)
-        if (lane == 63) listed[wave] = before;
-        __syncthreads();
-        int count = 0;
-        for (int i = 0; i < 4; i++) { if (i < wave) before += listed[i]; count += listed[i]; }
-        before -= __popc(bits);
-        for (uint32_t left = bits; left; left &= left - 1) list[before++] = (uint16_t) (32 * tid + __builtin_ctz(left));
-        __syncthreads();
+    px_share(w_all, A.dyn ? px_share_of(w_all, 8, A.own_parts) : A.own_share, (int) part, from, to);
+    px_queries<DP>(A, q, (int) tok, head, g);
+    px_start(S);
+    for (int w = from; w < to; w += 64) {
+        const int at = w0 + min(w + lane, to - 1);
+        uint32_t bits = A.mask[(int64_t) tok * words + at];
+        if (w + lane >= to) bits = 0;
+        if (32 * at < prompt) bits &= ~0u << (prompt - 32 * at);                // (prompt - 32 * at < 32: at >= prompt / 32)
+        if (n_kv - 32 * at < 32) bits &= (1u << (n_kv - 32 * at)) - 1;
+        const int upto = (int) pi_wave_scan((uint32_t) __popc(bits)), count = __builtin_amdgcn_readlane(upto, 63);
+        int before = upto - __popc(bits);
+        for (uint32_t left = bits; left; left &= left - 1) list[before++] = (uint16_t) (32 * lane + __builtin_ctz(left));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const int first = 32 * (w0 + w);
-        px_walk<DP>(A, S, q, mine, kvh, wave, lane, count, [&](int i) __attribute__((always_inline)) { return first + list[i]; });
+        px_walk<DP>(A, S, q, mine, (int) kvh, 0, 32, lane, count, [&](int i) __attribute__((always_inline)) { return first + list[i]; });
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    px_meet<DP>(S, lds, wave, lane);
-    if (wave == 0) px_leave<DP>(A, S, A.prompt_parts + part, tok, head, in < A.group, g);
+    px_leave<DP>(A, S, A.prompt_parts + (int) part, (int) tok, head, in < A.group, g);
 }
 
 // The parts' sums over their joint maximum.  Four of a row's values to a thread and about every `groups`-th part, the threads of a row meet in LDS: with a wave per row and its parts one after the other the loads' latency was all the
@@ -396,9 +404,19 @@ static void px_plan(px_args & A) {
     A.row_blocks = wide ? (rows + 127) / 128 : (rows + 31) / 32;
     A.own_blocks = (A.group + 31) / 32;
     const int64_t units = (int64_t) A.kv * A.row_blocks, own = (int64_t) A.n_tok * A.kv * A.own_blocks;
-    const int span = A.n_kv - A.prompt / 32 * 32;
-    A.prompt_parts = A.prompt == 0 ? 0 : (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256));
-    A.own_parts = A.n_kv == A.prompt ? 0 : (int) std::max<int64_t>(1, std::min<int64_t>(target / own, (span + 511) / 512));
+    const int words = (A.n_kv + 31) / 32 - A.prompt / 32, run = wide ? 64 : 32;
+    // two workgroups a compute unit, of 256 cells and more each; of a token's own cells four waves' worth of them, 16 words of the mask and more each
+    A.prompt_parts = A.own_parts = 0;
+    A.prompt_share = A.own_share = 1;
+    if (A.prompt > 0) {
+        A.prompt_share = px_share_of(A.prompt, run, (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256)));
+        A.prompt_parts = (A.prompt + A.prompt_share - 1) / A.prompt_share;
+    }
+    if (A.n_kv > A.prompt) {
+        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(4 * target / own, (words + 15) / 16)));
+        A.own_parts = (words + A.own_share - 1) / A.own_share;
+    }
+    A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_row_blocks = px_divide_by(std::max(1, A.row_blocks)); A.by_own_blocks = px_divide_by(A.own_blocks); A.by_own_parts = px_divide_by(std::max(1, A.own_parts));
 }
 
 static int px_sizes(const char * what, int dim, int heads, int kv, int n_tok, int prompt, int n_kv) {
@@ -422,8 +440,8 @@ extern "C" size_t pi_op_prefix_attention_scratch_floats(int head_dim, int n_head
 }
 
 template <int DP> static int px_launch(const px_args & A, hipStream_t s) {
-    const int64_t blocks = (int64_t) A.kv * A.prompt_parts * A.row_blocks + (int64_t) A.n_tok * A.kv * A.own_blocks * A.own_parts;
-    if (blocks > 0x7fffffff) { pi_set_error("pi_op_prefix_attention: %lld workgroups", (long long) blocks); return -1; }
+    const int64_t own = (int64_t) A.n_tok * A.kv * A.own_blocks * A.own_parts, blocks = (int64_t) A.kv * A.prompt_parts * A.row_blocks + (own + 3) / 4;
+    if (blocks > 0x1fffffff || own > 0x3fffffff) { pi_set_error("pi_op_prefix_attention: %lld workgroups", (long long) blocks); return -1; }
     const int parts = A.prompt_parts + A.own_parts, nta = std::min(A.n_tok, PI_KT_MAXNT - 1), acct = pi_account_n_kv() > 0 ? pi_account_n_kv() : A.n_kv;
     const double bytes = 4.0 * acct * A.row + 6.0 * A.n_tok * A.heads * A.dim;
     if (blocks > 0) {
@@ -476,22 +494,24 @@ struct pm_args {
     const uint16_t * k; int64_t row;
     const uint32_t * mask; const float * lse; const int32_t * dyn;
     float c;
-    int dim, heads, kv, group, n_tok, prompt, n_kv, cell_blocks, row_parts;
+    int dim, heads, kv, group, n_tok, prompt, n_kv, cell_blocks, row_parts, row_share;
+    px_div by_group, by_kv, by_blocks;
     float decay, * parts, * mass;                            // [row part][key head][cell]; null: the result is whole
 };
 
 template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_mass(const pm_args A, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;
     constexpr int KS = px_lds<DP>::K, N = DP / 32, CH = DP / 8, STAGE = 64 * KS;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > 4 * 32 * 272 ? 2 * STAGE : 4 * 32 * 272];
     __shared__ float lse[2][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
     const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv), words = (A.n_kv + 31) / 32;
-    const int cb = blockIdx.x % A.cell_blocks, kvh = blockIdx.x / A.cell_blocks % A.kv, part = blockIdx.x / A.cell_blocks / A.kv;
+    const uint32_t up = px_quotient(blockIdx.x, A.by_blocks), part = px_quotient(up, A.by_kv);
+    const int cb = (int) (blockIdx.x - up * A.cell_blocks), kvh = (int) (up - part * A.kv);
     const int cells0 = cb * 256, mine = cells0 + wave * 64;
     if (cells0 >= n_kv) return;                              // (nothing of these cells is read or written: k_mass_merge stops there too)
     int r0, r1;
-    px_share(A.n_tok * A.group, 64, part, A.row_parts, r0, r1);
+    px_share(A.n_tok * A.group, A.row_share, (int) part, r0, r1);
     px_u32x4 key[2][DP / 16], qr[N];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -505,11 +525,12 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         for (int i = 0; i < N; i++) {
             // (past the head's end the keys are zero; what is multiplied there is the head's first values)
             const int x = i * 256 + tid, d = x % CH * 8, m = min(r + x / CH, r1 - 1);
-            qr[i] = *(const px_u32x4 *) (A.q + (int64_t) (m / A.group) * A.q_stride + (int64_t) (kvh * A.group + m % A.group) * A.dim + (d < A.dim ? d : 0));
+            const int t = (int) px_quotient((uint32_t) m, A.by_group);
+            qr[i] = *(const px_u32x4 *) (A.q + t * A.q_stride + (int64_t) (kvh * A.group + m - t * A.group) * A.dim + (d < A.dim ? d : 0));
         }
         if (tid < 64) {
-            const int m = min(r + tid, r1 - 1);
-            const float x = A.lse[(int64_t) (m / A.group) * A.heads + kvh * A.group + m % A.group];
+            const int m = min(r + tid, r1 - 1), t = (int) px_quotient((uint32_t) m, A.by_group);
+            const float x = A.lse[(int64_t) t * A.heads + kvh * A.group + m - t * A.group];
             next_lse = r + tid >= r1 || x == -INFINITY ? INFINITY : x * 1.44269504f;      // (a row that saw nothing gives nothing)
         }
     };
@@ -540,7 +561,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
                     if constexpr (with_mask) {
                         bits = 0;
                         if (base < n_kv) {
-                            if (base + 32 > prompt) bits = A.mask[(int64_t) (min(r + 32 * v + n, r1 - 1) / A.group) * words + base / 32];
+                            if (base + 32 > prompt) bits = A.mask[(int64_t) px_quotient((uint32_t) min(r + 32 * v + n, r1 - 1), A.by_group) * words + base / 32];
                             if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
                             if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
                         }
@@ -562,18 +583,22 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         if (masked) rows(std::true_type{}); else rows(std::false_type{});
         if (more) store(cur ^ 1);
     }
+    // a lane has 32 cells of one row of 32: through LDS, [row of 32][cell], to one cell a lane
+    __syncthreads();
+    float * const at = (float *) lds + wave * (32 * 68);        // (rows 68 floats apart: sixteen bytes further round the banks)
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float x = sum[u][i];
-            x += pi_partner<16>(x); x += pi_partner<8>(x); x += pi_partner<4>(x); x += pi_partner<2>(x); x += pi_partner<1>(x);
-            const int cell = mine + 32 * u + px_cell(i, g);
-            if (n == i && cell < n_kv) {
-                if (A.parts) A.parts[((int64_t) part * A.kv + kvh) * A.n_kv + cell] = x;
-                else A.mass[cell] = A.decay == 0.0f ? x : A.decay * A.mass[cell] + x;
-            }
-        }
+        for (int i = 0; i < 16; i += 4) *(px_f32x4 *) (at + n * 68 + 32 * u + px_cell(i, g)) = px_f32x4{ sum[u][i], sum[u][i + 1], sum[u][i + 2], sum[u][i + 3] };
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float x[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+    for (int i = 0; i < 32; i++) x[i & 3] += at[i * 68 + lane];
+    const float all = (x[0] + x[1]) + (x[2] + x[3]);
+    const int cell = mine + lane;
+    if (cell >= n_kv) return;
+    if (A.parts) A.parts[((int64_t) part * A.kv + kvh) * A.n_kv + cell] = all;
+    else A.mass[cell] = A.decay == 0.0f ? all : A.decay * A.mass[cell] + all;
 }
 
 __global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, const int32_t * __restrict__ abort_w) {
@@ -595,6 +620,9 @@ static void pm_plan(pm_args & A) {
     A.row_parts = 1;
     double least = 1e30;
     for (int p = 1; p <= 16 && p <= (rows + 63) / 64; p++) { const double t = (double) ((units * p + slots - 1) / slots) * (1.0 / p + 0.03); if (t < least * 0.98) { least = t; A.row_parts = p; } }
+    A.row_share = px_share_of(std::max(1, rows), 64, A.row_parts);
+    A.row_parts = std::max(1, (rows + A.row_share - 1) / A.row_share);
+    A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_blocks = px_divide_by(std::max(1, A.cell_blocks));
 }
 static size_t pm_floats(const pm_args & A) { const size_t parts = (size_t) A.kv * A.row_parts; return parts > 1 ? parts * A.n_kv : 0; }
 
