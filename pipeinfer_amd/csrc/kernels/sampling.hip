@@ -43,47 +43,47 @@
 #define SP_MAX_VOCAB (1 << 19)
 
 typedef unsigned long long sp_u64;
-// e^x, x <= 0 (or a little above): x = n ln 2 / 64 + r, 2^(n / 64) from a table of 64 (sp_table) and the exponent, e^r by its series up to r^4 / 24, |r| <= 0.0055 (the next term: 4e-14).  A third of the instructions less than without a table
-#define SP_TABLE 64
+// e^x, x <= 0 (or a little above): x = n ln 2 / 256 + r, 2^(n / 256) from a table (sp_table) and the exponent, e^r by its series up to r^3 / 6, |r| <= 0.00136 (the next term: 1.4e-13)
+#define SP_TABLE 256
+static __device__ __forceinline__ double sp_scaled(double s, double p, int n) {      // s 2^(n / 256): the table's value p with another exponent
+    return s * __builtin_bit_cast(double, __builtin_bit_cast(sp_u64, p) + ((sp_u64) (uint32_t) ((n >> 8) << 20) << 32));
+}
 static __device__ __forceinline__ double sp_exp(double x, const double * table) {
     x = fmax(x, -600.0);                                     // (1e-260 for nothing: a choice of 0 instead would be a branch, and every exponential would wait for the one before)
-    const double t = fma(x, 92.332482616893656877, 0x1.8p52), r = fma(t - 0x1.8p52, -0.010830424696249145459, x);          // (n: the low bits of t)
+    const double t = fma(x, 369.32993046757462871, 0x1.8p52), r = fma(t - 0x1.8p52, -0.0027076061740622863649, x);          // (n: the low bits of t)
     const int n = (int) (uint32_t) __builtin_bit_cast(sp_u64, t);
-    const double s = fma(fma(fma(fma(1.0 / 24.0, r, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0), p = table[n & 63];
-    return s * __builtin_bit_cast(double, __builtin_bit_cast(sp_u64, p) + ((sp_u64) (uint32_t) ((n >> 6) << 20) << 32));    // (2^(n / 64): the table's value with another exponent)
+    return sp_scaled(fma(fma(fma(1.0 / 6.0, r, 0.5), r, 1.0), r, 1.0), table[n & 255], n);
 }
-// four of them side by side: one by one their latency - a dozen dependent fp64 instructions and the table, 350 clocks - is all the time
+// four of them (x >= -600) side by side: one by one their latency - a dozen dependent fp64 instructions and the table, 350 clocks - is all the time
 static __device__ __forceinline__ void sp_exp4(const double (&x)[4], double (&y)[4], const double * table) {
     double t[4], r[4], p[4], s[4];
     int n[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) { r[e] = fmax(x[e], -600.0); t[e] = fma(r[e], 92.332482616893656877, 0x1.8p52); }
+    for (int e = 0; e < 4; e++) t[e] = fma(x[e], 369.32993046757462871, 0x1.8p52);
 #pragma unroll
-    for (int e = 0; e < 4; e++) { n[e] = (int) (uint32_t) __builtin_bit_cast(sp_u64, t[e]); p[e] = table[n[e] & 63]; r[e] = fma(t[e] - 0x1.8p52, -0.010830424696249145459, r[e]); }
+    for (int e = 0; e < 4; e++) { n[e] = (int) (uint32_t) __builtin_bit_cast(sp_u64, t[e]); p[e] = table[n[e] & 255]; r[e] = fma(t[e] - 0x1.8p52, -0.0027076061740622863649, x[e]); }
 #pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = fma(1.0 / 24.0, r[e], 1.0 / 6.0);
-#pragma unroll
-    for (int e = 0; e < 4; e++) s[e] = fma(s[e], r[e], 0.5);
+    for (int e = 0; e < 4; e++) s[e] = fma(1.0 / 6.0, r[e], 0.5);
 #pragma unroll
     for (int e = 0; e < 4; e++) s[e] = fma(s[e], r[e], 1.0);
 #pragma unroll
     for (int e = 0; e < 4; e++) s[e] = fma(s[e], r[e], 1.0);
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = s[e] * __builtin_bit_cast(double, __builtin_bit_cast(sp_u64, p[e]) + ((sp_u64) (uint32_t) ((n[e] >> 6) << 20) << 32));
+    for (int e = 0; e < 4; e++) y[e] = sp_scaled(s[e], p[e], n[e]);
 }
-// 2^(i / 64) by the series of e^(i ln 2 / 64 - ln 2 / 2) up to its 15th power, times the root of two (by the first 64 threads)
+// 2^(i / 256) by the series of e^(i ln 2 / 256 - ln 2 / 2) up to its 15th power, times the root of two (by the first 256 threads)
 static __device__ __forceinline__ void sp_table(double * table) {
     const int i = threadIdx.x;
     if (i >= SP_TABLE) return;
-    const double x = (double) (i - 32) * 0.010830424696249145459;
+    const double x = (double) (i - 128) * 0.0027076061740622863649;
     double s = 1.0;
 #pragma unroll
     for (int k = 15; k > 0; k--) s = fma(s * x, 1.0 / (double) k, 1.0);
     table[i] = s * 1.4142135623730950488;
 }
-// in steps: as the fraction of a double of 2^52; as a whole number in a double (up to 2^9 of them add up exactly)
+// in steps: a weight, as the fraction of a double of 2^52; a sum of weights
 static __device__ __forceinline__ sp_u64 sp_steps(double w) { return __builtin_bit_cast(sp_u64, fma(w, SP_ONE, 0x1p52)) & 0xfffffffffffffull; }
-static __device__ __forceinline__ double sp_whole(double w) { return fma(w, SP_ONE, 0x1p52) - 0x1p52; }
+static __device__ __forceinline__ sp_u64 sp_sum_steps(double sum) { return (sp_u64) (sum * SP_ONE + 0.5); }
 
 // larger value first, then the lower id; 0: not there
 static __device__ __forceinline__ sp_u64 sp_rank(float x, int id) {
@@ -206,9 +206,10 @@ template <class F> static __device__ __forceinline__ int sp_reach(sp_shared & L,
     return L.hit;
 }
 
-// the token in the values [from, to), of which `t` of the sum is left
+// the token in the values [from, to), of which `t` of the sum is left.  (A run's sum may be a few steps above its values': then it is the last of them)
 static __device__ __forceinline__ void sp_pick(const sp_args & A, const sp_row & R, int row, int from, int to, sp_u64 t, sp_u64 sum, int kept) {
     const int lane = threadIdx.x & 63;
+    int last = -1;
     for (int i0 = from; i0 < to; i0 += 64) {
         const int i = i0 + lane;
         const float v = i < to ? R.x[i] : -INFINITY;
@@ -219,7 +220,10 @@ static __device__ __forceinline__ void sp_pick(const sp_args & A, const sp_row &
             return;
         }
         t -= all;
+        const unsigned long long who = __ballot(mine > 0);
+        if (who) last = i0 + 63 - __builtin_clzll(who);
     }
+    if (lane == 0 && last >= 0) sp_leave(A, row, last, R.part(R.x[last], sum), kept);
 }
 // the same for a run of values whose sum is held: the workgroup's waves take a sixteenth each
 static __device__ __forceinline__ void sp_pick_run(const sp_args & A, const sp_row & R, sp_shared & L, int row, int from, int to, sp_u64 t, sp_u64 sum, int kept) {
@@ -231,8 +235,9 @@ static __device__ __forceinline__ void sp_pick_run(const sp_args & A, const sp_r
     __syncthreads();
     if (lane == 0) L.waves[wave] = e;
     __syncthreads();
-    int sub = 0;
-    while (sub < SP_WAVES - 1 && t >= L.waves[sub]) t -= L.waves[sub++];
+    int sub = 0, last = 0;
+    for (int i = 0; i < SP_WAVES; i++) if (L.waves[i] > 0) last = i;
+    while (sub < last && t >= L.waves[sub]) t -= L.waves[sub++];
     if (wave == sub) sp_pick(A, R, row, a, b, t, sum, kept);
 }
 
@@ -802,7 +807,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
     if (tid == 0) *rest = sp_rest{ best, zero, lo == 0 ? INFINITY : zero - (float) lo / SP_COARSE_UNIT, zero - ((float) hi + 1.5f) / SP_COARSE_UNIT, 1, joined, 0 };
 }
 
-// Bound by its instructions: 45 a value, of which the two exponentials are 30 (64 rows of 131072: 90 a value, with the bins found again, took 29 us)
+// Sums of a run in fp64, in an order that is always the same, then in steps.  Bound by its instructions, the fp64 ones for the most part: 22 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, 25 us)
 template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
     const sp_rest rest = S.rest[row];
@@ -838,33 +843,30 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
         for (int run = 0; run < 2; run++) {
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                double d[4], w[4], c[4];
+                double d[4], w[4];
                 bool stays[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) { const float v = run ? x[8 + 4 * half + e] : x[4 * half + e]; d[e] = (double) v - top; stays[e] = v > rest.above; }
-                sp_exp4(d, w, table);                        // (nothing: 0 steps)
+                for (int e = 0; e < 4; e++) { const float v = run ? x[8 + 4 * half + e] : x[4 * half + e]; d[e] = fmax((double) v - top, -600.0); stays[e] = v > rest.above; }
+                sp_exp4(d, w, table);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    c[e] = sp_whole(w[e]);
-                    all += c[e]; above += stays[e] ? c[e] : 0.0;
+                    all += w[e]; above += stays[e] ? w[e] : 0.0;
                     stays[e] = stays[e] && (!few_stay || w[e] >= (double) R.min_p);
                     kept += __popcll(__ballot(stays[e]));
                 }
                 if (!once && !R.greedy) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) d[e] *= R.cooled;
+                    for (int e = 0; e < 4; e++) d[e] = fmax(d[e] * R.cooled, -600.0);
                     sp_exp4(d, w, table);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) c[e] = sp_whole(w[e]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) chance += stays[e] ? c[e] : 0.0;
+                for (int e = 0; e < 4; e++) chance += stays[e] ? w[e] : 0.0;
             }
-            const sp_u64 c = sp_wave_sum((sp_u64) chance);
+            const sp_u64 c = sp_sum_steps(pi_wave_sum_f64(chance));
             if (lane == 0) mine->chances[2 * wave + run] = c;
             chance = 0.0;
         }
-        const sp_u64 a = sp_wave_sum((sp_u64) all), b = sp_wave_sum((sp_u64) above);
+        const sp_u64 a = sp_sum_steps(pi_wave_sum_f64(all)), b = sp_sum_steps(pi_wave_sum_f64(above));
         if (lane == 0) { sums[wave][0] = a; sums[wave][1] = b; sums[wave][2] = (sp_u64) kept; }
     }
     __syncthreads();
@@ -877,7 +879,7 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
 }
 
 // the slices of a row; false: they do not say enough
-static __device__ __forceinline__ bool sp_join(const sp_args & A, sp_row & R, sp_shared & L, int row, const sp_slice * mine, const sp_u64 * lists, int slices, bool border) {
+static __device__ __forceinline__ bool sp_join(const sp_args & A, sp_row & R, sp_shared & L, int row, const sp_slice * mine, const sp_u64 * lists, int slices, bool border, float above_v, float least) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // (every wave for itself: a lane has a slice)
     static_assert(SP_MAX_VOCAB / SP_SLICE <= 64, "");
@@ -897,32 +899,38 @@ static __device__ __forceinline__ bool sp_join(const sp_args & A, sp_row & R, sp
         return true;
     }
     if (border) {
-        // the rank of the border: ranked by counting where that is the quicker way, else in order
+        // the border's rank: the list's weights in 512 bins of their own, and the ranks inside the one that the border is in
         const double want = (double) R.top_p * (double) weights;
         const sp_u64 target = min(want >= 1.0 ? (sp_u64) __builtin_ceil(want) : 1, weights);
         if (above >= target) return false;
-        for (int i = tid; i < n; i += SP_THREADS) { const sp_u64 r = L.list[i]; L.weight[2 * i] = r; L.weight[2 * i + 1] = sp_steps(R.weight(sp_value(r))); }
+        const float from = fminf(above_v, R.top), scale = 512.0f / fmaxf(from - least, 1e-30f);
+        auto bin = [&](float v) __attribute__((always_inline)) { return (int) __builtin_amdgcn_fmed3f((from - v) * scale, 0.0f, 511.0f); };
+        if (tid < 512) L.weight[tid] = 0;
+        if (tid == 0) { L.n = 0; L.hit = -1; }
         __syncthreads();
-        sp_u64 most = 0;
-        if (n <= SP_RANKED) {
-            if (tid < n) {
-                const sp_u64 r = L.weight[2 * tid];
-                sp_u64 sum = above;
-#pragma unroll 8
-                for (int o = 0; o < n; o++) { const ulonglong2 x = *(const ulonglong2 *) &L.weight[2 * o]; sum += x.x > r ? x.y : 0; }
-                if (sum < target) atomicMin(&L.answer, r);
-                most = sum + L.weight[2 * tid + 1];
-            }
-        } else {
-            sp_sort(L.list, n);
-            sp_u64 own[SP_LIST / SP_THREADS], s = 0, all;
-#pragma unroll
-            for (int i = 0; i < SP_LIST / SP_THREADS; i++) { const int at = SP_LIST / SP_THREADS * tid + i; own[i] = at < n ? sp_steps(R.weight(sp_value(L.list[at]))) : 0; s += own[i]; }
-            sp_u64 sum = above + sp_before(s, L, lane, wave, all);
-#pragma unroll
-            for (int i = 0; i < SP_LIST / SP_THREADS; i++) { const int at = SP_LIST / SP_THREADS * tid + i; if (at < n && sum < target) atomicMin(&L.answer, L.list[at]); sum += own[i]; if (at < n) most = sum; }
+        for (int i = tid; i < n; i += SP_THREADS) { const float v = sp_value(L.list[i]); atomicAdd(&L.weight[bin(v)], sp_steps(R.weight(v))); }
+        __syncthreads();
+        sp_u64 all;
+        const sp_u64 mine_w = tid < 512 ? L.weight[tid] : 0, ahead = above + sp_before(mine_w, L, lane, wave, all);
+        if (tid < 512 && ahead < target && ahead + mine_w >= target) { L.hit = tid; L.before = ahead; }
+        __syncthreads();
+        if (L.hit < 0) return false;
+        const int hit = L.hit;
+        const sp_u64 base = L.before;
+        for (int i = tid; i < n; i += SP_THREADS) {
+            const sp_u64 r = L.list[i];
+            if (bin(sp_value(r)) == hit) { const int at = atomicAdd(&L.n, 1); L.weight[2 * at] = r; L.weight[2 * at + 1] = sp_steps(R.weight(sp_value(r))); }
         }
-        if (!__syncthreads_or(most >= target)) return false;
+        __syncthreads();
+        const int m = L.n;
+        for (int i = tid; i < m; i += SP_THREADS) {
+            const sp_u64 r = L.weight[2 * i];
+            sp_u64 sum = base;
+#pragma unroll 4
+            for (int o = 0; o < m; o++) { const ulonglong2 x = *(const ulonglong2 *) &L.weight[2 * o]; sum += x.x > r ? x.y : 0; }
+            if (sum < target) atomicMin(&L.answer, r);
+        }
+        __syncthreads();
         R.last = L.answer;
     }
     if (R.greedy) {                                          // (the first; how many stay is all there is to say)
@@ -963,7 +971,7 @@ template <bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sample_join
     sp_row R(A, row, L.table);
     if (rest.joined != 0) R.known(rest.best);
     sp_table(L.table);
-    if (rest.joined != 0 && sp_join(A, R, L, row, S.slices + (int64_t) row * slices, S.lists + (int64_t) row * slices * SP_SLICE_LIST, slices, R.nucleus())) return;
+    if (rest.joined != 0 && sp_join(A, R, L, row, S.slices + (int64_t) row * slices, S.lists + (int64_t) row * slices * SP_SLICE_LIST, slices, R.nucleus(), rest.above, rest.listed)) return;
     __syncthreads();
     const sp_values<0, WIDE> X(R.x, R.V);
     sp_u64 best = 0;
