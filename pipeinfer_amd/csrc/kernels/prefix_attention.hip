@@ -42,21 +42,34 @@ template <int DP> static __device__ __forceinline__ void px_start(px_sums<DP> & 
     S.m = -INFINITY; S.l = 0.0f;
 }
 
-// a tile of 32 cells, of which the first `live` count: key(i) gives the operand of its values 16 i + 8 g .., value(j, z) that of the outputs 32 j .. and the cells 16 z ..; c = scale * log2(e)
-template <int DP, class K, class V> static __device__ __forceinline__ void px_tile(px_sums<DP> & S, const px_u32x4 (&q)[DP / 16], float c, int live, int g, K && key, V && value) {
-    px_f32x16 s = px_zero();
+// scores of which the first `live` cells of the tile count
+static __device__ __forceinline__ void px_only(px_f32x16 & s, int live, int g) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) s = px_mfma(key(i), q[i], s);
-    if (live < 32) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) if (px_cell(i, g) >= live) s[i] = -INFINITY;
-    }
-    float p[16], l;
+    for (int i = 0; i < 16; i++) if (px_cell(i, g) >= live) s[i] = -INFINITY;
+}
+
+// a tile's weights, as operands of the products with the values: what a weight's first fp16 leaves in a second one
+struct px_weights { px_u32x4 hi[2], lo[2]; };
+static __device__ __forceinline__ void px_no_weights(px_weights & P) { for (int z = 0; z < 2; z++) P.hi[z] = P.lo[z] = px_u32x4{ 0, 0, 0, 0 }; }
+
+// of a tile's scores the weights and their sum; c = scale * log2(e).  S holds the products of the tiles before
+template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & S, px_weights & P, const px_f32x16 & s, float c) {
+    float p[16], l, minus = -1.0f;
+    asm("" : "+v"(minus));                                   // (unknown to the compiler: a - h would be a conversion and a subtraction, fma takes the fp16 as it is)
     auto weigh = [&]() __attribute__((always_inline)) {
         const float lift = PX_LIFT - (S.m == -INFINITY ? 0.0f : S.m);
 #pragma unroll
         for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, lift));
         l = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) + (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float a = p[8 * z + 2 * e], b = p[8 * z + 2 * e + 1];
+                const px_half2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
+                P.hi[z][e] = __builtin_bit_cast(uint32_t, h);
+                P.lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], minus, a), fmaf((float) h[1], minus, b)));
+            }
     };
     weigh();
     // (the maximum is looked for where a lane's weights say that it has grown, or that there was none: it costs a dozen instructions a tile)
@@ -75,26 +88,6 @@ template <int DP, class K, class V> static __device__ __forceinline__ void px_ti
         weigh();
     }
     S.l += l;
-    float minus = -1.0f;
-    asm("" : "+v"(minus));                                   // (unknown to the compiler: a - h would be a conversion and a subtraction, fma takes the fp16 as it is)
-    px_u32x4 hi[2], lo[2];
-#pragma unroll
-    for (int z = 0; z < 2; z++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float a = p[8 * z + 2 * e], b = p[8 * z + 2 * e + 1];
-            const px_half2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
-            hi[z][e] = __builtin_bit_cast(uint32_t, h);
-            lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], minus, a), fmaf((float) h[1], minus, b)));
-        }
-#pragma unroll
-    for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-        for (int z = 0; z < 2; z++) {
-            const px_u32x4 v = value(j, z);
-            S.acc[j] = px_mfma(v, hi[z], S.acc[j]);
-            S.acc[j] = px_mfma(v, lo[z], S.acc[j]);
-        }
 }
 
 // the values' operand from rows of `stride` bytes in LDS: at = the wave's first row + px_value_at; sixteen lanes take four rows of sixteen values and each gets a column
@@ -104,6 +97,18 @@ template <int STRIDE> static __device__ __forceinline__ px_u32x4 px_value(const 
     const px_u32x2 a = __builtin_bit_cast(px_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + 16 * z * STRIDE + 64 * j)));
     const px_u32x2 b = __builtin_bit_cast(px_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *) (at + (16 * z + 8) * STRIDE + 64 * j)));
     return px_u32x4{ a[0], a[1], b[0], b[1] };
+}
+
+// the products of a tile's weights with its values, whose first row is px_value_at behind `at`
+template <int DP, int VS> static __device__ __forceinline__ void px_products(px_sums<DP> & S, const px_weights & P, const uint8_t * at) {
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            const px_u32x4 v = px_value<VS>(at, j, z);
+            S.acc[j] = px_mfma(v, P.hi[z], S.acc[j]);
+            S.acc[j] = px_mfma(v, P.lo[z], S.acc[j]);
+        }
 }
 
 // n / d for n < 2^31 (a division by what only the arguments know is thirty instructions, and a kernel that runs for a few us waits for every line of code that it has not run yet: 80 clocks for 64 bytes)
@@ -161,10 +166,11 @@ template <int DP> static __device__ __forceinline__ void px_queries(const px_arg
     for (int i = 0; i < DP / 16; i++) q[i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (row + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
 }
 
-// Many rows: a wave has 32 of the workgroup's 128, all walk the same cells.  Tiles of 64 cells, two in LDS: while one is worked on the next is on its way in registers
+// Many rows: a wave has 32 of the workgroup's 128, all walk the same cells, 32 at a time through a ring of four tiles in LDS.  Three tiles are in work at once, so that the matrix cores and the vector unit are: while the weights of tile t are
+// made from its scores, the products of the weights of t - 1 with the values and of the keys of t + 1 with the queries run; tile t + 2 goes to LDS and t + 3 is on its way in registers
 template <int DP> static __device__ __forceinline__ void px_wide(const px_args & A, uint8_t * lds, int kvh, int block, int part, int c0, int c1) {
-    constexpr int KS = px_lds<DP>::K, VS = px_lds<DP>::V, STAGE = 64 * (KS + VS), N = DP / 32, CH = DP / 8;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5, rows = A.n_tok * A.group;
+    constexpr int KS = px_lds<DP>::K, VS = px_lds<DP>::V, TILE = 32 * (KS + VS), CH = DP / 8, N = (32 * CH + 255) / 256;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5, rows = A.n_tok * A.group, tiles = (c1 - c0 + 31) / 32;
     const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group), head = kvh * A.group + at - tok * A.group;
     px_u32x4 q[DP / 16], kr[N], vr[N];
     px_queries<DP>(A, q, tok, head, g);
@@ -172,42 +178,54 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
     px_start(S);
     const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
     // (a chunk past the head's end reads its first: the queries are zero there, and such outputs do not leave)
-    auto load = [&](int c) __attribute__((always_inline)) {
-        const uint16_t * kc = k + (int64_t) c * A.row, * vc = v + (int64_t) c * A.row;
-        const int last = c1 - 1 - c;
+    auto load = [&](int t) __attribute__((always_inline)) {
+        const int64_t c = c0 + 32 * t;
+        const uint16_t * kc = k + c * A.row, * vc = v + c * A.row;
+        const int last = c1 - 1 - c0 - 32 * t;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int x = i * 256 + tid, d = x % CH * 8;
-            const uint32_t o = (uint32_t) (last >= 63 ? x / CH : min(x / CH, last)) * (uint32_t) A.row + (uint32_t) (d < A.dim ? d : 0);
+            const int x = min(i * 256 + tid, 32 * CH - 1), d = x % CH * 8;
+            const uint32_t o = (uint32_t) (last >= 31 ? x / CH : min(x / CH, last)) * (uint32_t) A.row + (uint32_t) (d < A.dim ? d : 0);
             kr[i] = *(const px_u32x4 *) (kc + o);
             vr[i] = *(const px_u32x4 *) (vc + o);
         }
     };
-    auto store = [&](uint8_t * to) __attribute__((always_inline)) {
+    auto store = [&](int t) __attribute__((always_inline)) {
+        uint8_t * to = lds + (t & 3) * TILE;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int x = i * 256 + tid;
+            const int x = min(i * 256 + tid, 32 * CH - 1);
             *(px_u32x4 *) (to + x / CH * KS + x % CH * 16) = kr[i];
-            *(px_u32x4 *) (to + 64 * KS + x / CH * VS + x % CH * 16) = vr[i];
+            *(px_u32x4 *) (to + 32 * KS + x / CH * VS + x % CH * 16) = vr[i];
         }
     };
-    load(c0);
-    store(lds);
-    int cur = 0;
-    for (int c = c0; c < c1; c += 64, cur ^= 1) {
-        __syncthreads();
-        const bool more = c + 64 < c1;
-        if (more) load(c + 64);
-        const uint8_t * st = lds + cur * STAGE;
+    auto scores = [&](int t) __attribute__((always_inline)) {
+        const uint8_t * kt = lds + (t & 3) * TILE + n * KS + 16 * g;
+        px_f32x16 s = px_zero();
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (c + 32 * u >= c1) continue;
-            const uint8_t * kt = st + (32 * u + n) * KS + 16 * g, * vt = st + 64 * KS + 32 * u * VS + px_value_at(lane, VS);
-            px_tile<DP>(S, q, A.c, c1 - c - 32 * u, g, [&](int i) __attribute__((always_inline)) { return *(const px_u32x4 *) (kt + 32 * i); },
-                        [&](int j, int z) __attribute__((always_inline)) { return px_value<VS>(vt, j, z); });
-        }
-        if (more) store(lds + (cur ^ 1) * STAGE);
+        for (int i = 0; i < DP / 16; i++) s = px_mfma(*(const px_u32x4 *) (kt + 32 * i), q[i], s);
+        return s;
+    };
+    load(0); store(0);
+    if (tiles > 1) { load(1); store(1); }
+    if (tiles > 2) load(2);
+    __syncthreads();
+    px_f32x16 s = scores(0);
+    px_weights P;
+    px_no_weights(P);
+    const int value_at = 32 * KS + px_value_at(lane, VS);
+    for (int t = 0; t < tiles; t++) {
+        if (t > 0) __syncthreads();
+        if (t + 2 < tiles) store(t + 2);
+        if (t + 3 < tiles) load(t + 3);
+        if (c0 + 32 * t + 32 > c1) px_only(s, c1 - c0 - 32 * t, g);
+        // (of the first tile no weights: its own values times 0; behind the last one the scores of whatever stands there, for nobody)
+        px_products<DP, VS>(S, P, lds + (max(t - 1, 0) & 3) * TILE + value_at);
+        const px_f32x16 next = scores(t + 1);
+        px_weigh<DP>(S, P, s, A.c);
+        s = next;
     }
+    px_products<DP, VS>(S, P, lds + (tiles - 1 & 3) * TILE + value_at);
     px_leave<DP>(A, S, part, tok, head, row < rows, g);
 }
 
@@ -241,7 +259,13 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         if (at + step < count) load(at + step);
         const uint8_t * vt = mine + px_value_at(lane, VS);
-        px_tile<DP>(S, q, A.c, count - at, g, [&](int i) __attribute__((always_inline)) { return kc[i]; }, [&](int j, int z) __attribute__((always_inline)) { return px_value<VS>(vt, j, z); });
+        px_f32x16 s = px_zero();
+#pragma unroll
+        for (int i = 0; i < N; i++) s = px_mfma(kc[i], q[i], s);
+        if (at + 32 > count) px_only(s, count - at, g);
+        px_weights P;
+        px_weigh<DP>(S, P, s, A.c);
+        px_products<DP, VS>(S, P, vt);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
@@ -289,7 +313,7 @@ static __host__ __device__ __forceinline__ int px_share_of(int n, int run, int p
 
 template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;                      // (what a wave takes from LDS as an index, it has put there itself)
-    constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 2 * 64 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
+    constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 4 * 32 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
     __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? NARROW : WIDE_B];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
     const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv);
@@ -302,7 +326,7 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
         const uint32_t b = blockIdx.x, eights = pairs % 8 == 0, of = eights ? b >> 3 : b, by = px_quotient(of, A.by_row_blocks), block = of - by * A.row_blocks, pair = eights ? by * 8 + (b & 7) : by;
         const uint32_t part = px_quotient(pair, A.by_kv), kvh = pair - part * A.kv;
         int c0, c1;
-        px_share(prompt, A.dyn ? px_share_of(prompt, WIDE ? 64 : 32, A.prompt_parts) : A.prompt_share, (int) part, c0, c1);
+        px_share(prompt, A.dyn ? px_share_of(prompt, 32, A.prompt_parts) : A.prompt_share, (int) part, c0, c1);
         const int rows = A.n_tok * A.group;
         if constexpr (WIDE) {
             if (c0 >= c1) {                                  // (fewer cells than there may be)
@@ -404,16 +428,17 @@ static void px_plan(px_args & A) {
     A.row_blocks = wide ? (rows + 127) / 128 : (rows + 31) / 32;
     A.own_blocks = (A.group + 31) / 32;
     const int64_t units = (int64_t) A.kv * A.row_blocks, own = (int64_t) A.n_tok * A.kv * A.own_blocks;
-    const int words = (A.n_kv + 31) / 32 - A.prompt / 32, run = wide ? 64 : 32;
+    const int words = (A.n_kv + 31) / 32 - A.prompt / 32;
     // two workgroups a compute unit, of 256 cells and more each; of a token's own cells four waves' worth of them, 16 words of the mask and more each
     A.prompt_parts = A.own_parts = 0;
     A.prompt_share = A.own_share = 1;
     if (A.prompt > 0) {
-        A.prompt_share = px_share_of(A.prompt, run, (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256)));
+        A.prompt_share = px_share_of(A.prompt, 32, (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256)));
         A.prompt_parts = (A.prompt + A.prompt_share - 1) / A.prompt_share;
     }
     if (A.n_kv > A.prompt) {
-        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(4 * target / own, (words + 15) / 16)));
+        const int64_t left = std::max<int64_t>(4 * (target - A.prompt_parts * units), own);          // (waves of workgroups that run beside the prompt's)
+        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(left / own, (words + 15) / 16)));
         A.own_parts = (words + A.own_share - 1) / A.own_share;
     }
     A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_row_blocks = px_divide_by(std::max(1, A.row_blocks)); A.by_own_blocks = px_divide_by(A.own_blocks); A.by_own_parts = px_divide_by(std::max(1, A.own_parts));
