@@ -28,7 +28,7 @@ def test_attention_refuses(args, why):
 @pytest.mark.parametrize("call,why", [
     (lambda lib, mass: mass(dim=12), b"steps of 8"), (lambda lib, mass: mass(prompt=500), b"500 of"), (lambda lib, mass: mass(lse=None), b"are NULL"), (lambda lib, mass: mass(mass=None), b"are NULL"),
     (lambda lib, mass: mass(k=None), b"are NULL"), (lambda lib, mass: mass(mask=None), b"are NULL"), (lambda lib, mass: mass(q=P + 2), b"16 bytes"), (lambda lib, mass: mass(stride=511), b"511"), (lambda lib, mass: mass(decay=float("nan")), b"decay"),
-    (lambda lib, mass: mass(scale=float("inf")), b"scale"), (lambda lib, mass: mass(scratch=None), b"0 floats"), (lambda lib, mass: mass(floats=3), b"3 floats"),
+    (lambda lib, mass: mass(scale=float("inf")), b"scale"), (lambda lib, mass: mass(scale=0.0), b"scale 0"), (lambda lib, mass: mass(scale=-0.1), b"scale -0.1"), (lambda lib, mass: mass(scratch=None), b"0 floats"), (lambda lib, mass: mass(floats=3), b"3 floats"),
     (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 11, P, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, -1, P, None), b"-1 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(None, None, 10, 4, P, None), b"is NULL"),
     (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 4, None, None), b"is NULL"),
     (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, P, 11, 10, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_move(None, None, 1, P, 4, 10, None), b"is NULL"),
