@@ -127,7 +127,7 @@ struct px_args {
     float c;
     int dim, heads, kv, group, n_tok, prompt, n_kv;
     int row_blocks, prompt_parts, own_blocks, own_parts;     // of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
-    px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts;
+    px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts, by_parts, by_quads;
     int prompt_share, own_share;                             // cells, words of the mask of a part where the sizes are the arguments'
     float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
     float * out; int64_t out_stride; float * lse;
@@ -370,15 +370,15 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
     px_leave<DP>(A, S, A.prompt_parts + (int) part, (int) tok, head, in < A.group, g);
 }
 
+#define PX_PARTS 1088                                            /* what k_prefix_merge has room for; the prompt takes two of a compute unit's at most */
 // The parts' sums over their joint maximum.  Four of a row's values to a thread and about every `groups`-th part, the threads of a row meet in LDS: with a wave per row and its parts one after the other the loads' latency was all the
 // time (4096 rows of 17 parts: 24.2 us; 1024 of 17: 20.8)
-#define PX_MERGED 1088
-__global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, int groups, int rows_here, const int32_t * __restrict__ abort_w) {
+__global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, int log_groups, int rows_here, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;
-    __shared__ float2 ml[PX_MERGED];
+    __shared__ float2 ml[PX_PARTS];                         // (512 of them at most where the workgroup has more than one row)
     __shared__ px_f32x4 sums[256];
     __shared__ float ls[256];
-    const int tid = threadIdx.x, quads = A.dim / 4, at = tid / quads, d = 4 * (tid % quads), mine = at / groups, grp = at % groups;
+    const int tid = threadIdx.x, quads = A.dim / 4, at = (int) px_quotient((uint32_t) tid, A.by_quads), d = 4 * (tid - at * quads), mine = at >> log_groups, groups = 1 << log_groups, grp = at & (groups - 1);
     const int64_t rows = (int64_t) A.n_tok * A.heads, r0 = (int64_t) blockIdx.x * rows_here;
     const bool on = mine < rows_here && r0 + mine < rows;
     const float * from = A.parts_o + min(r0 + mine, rows - 1) * A.dim + d;
@@ -389,21 +389,32 @@ __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts
         for (int i = 0; i < 4; i++) x[i] = *(const px_f32x4 *) (from + min(p + i * groups, parts - 1) * step);
     };
     if (parts > 0) load(grp);
-    for (int i = tid; i < rows_here * parts; i += 256) ml[i] = A.parts_ml[i % parts * rows + min(r0 + i / parts, rows - 1)];
+    for (int i = tid; i < rows_here * parts; i += 256) {
+        const int of = (int) px_quotient((uint32_t) i, A.by_parts);
+        float2 v = A.parts_ml[(i - of * parts) * rows + min(r0 + of, rows - 1)];
+        if (v.y == 0.0f) v.x = -INFINITY;                    // (a part without a cell: its outputs are not there)
+        ml[i] = v;
+    }
     __syncthreads();
     float m = -INFINITY, l = 0.0f;
     px_f32x4 o = { 0.0f, 0.0f, 0.0f, 0.0f };
     if (on) {
-        for (int p = 0; p < parts; p++) { const float2 v = ml[mine * parts + p]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
+        const float2 * of = ml + mine * parts;
+#pragma unroll 1
+        for (int p = 0; p < parts; p += 8)
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, of[min(p + i, parts - 1)].x);
+        const float from_m = m == -INFINITY ? 0.0f : m;
         for (int p = grp; p < parts; p += 4 * groups) {
             if (p != grp) load(p);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (p + i * groups >= parts) continue;
-                const float2 v = ml[mine * parts + p + i * groups];
-                if (v.y == 0.0f) continue;                   // (a part without a cell: its outputs are not there)
-                const float f = __builtin_amdgcn_exp2f(v.x - m);
-                l += v.y * f; o += x[i] * f;
+                float2 v = of[min(p + i * groups, parts - 1)];
+                if (p + i * groups >= parts) v.y = 0.0f;
+                const float f = __builtin_amdgcn_exp2f(v.x - from_m);
+                l += v.y * f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] += v.y == 0.0f ? 0.0f : x[i][e] * f;
             }
         }
     }
@@ -429,19 +440,24 @@ static void px_plan(px_args & A) {
     A.own_blocks = (A.group + 31) / 32;
     const int64_t units = (int64_t) A.kv * A.row_blocks, own = (int64_t) A.n_tok * A.kv * A.own_blocks;
     const int words = (A.n_kv + 31) / 32 - A.prompt / 32;
-    // two workgroups a compute unit, of 256 cells and more each; of a token's own cells four waves' worth of them, 16 words of the mask and more each
+    // Of the prompt two workgroups a compute unit where each has 1024 cells and more (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 129 us, with one 139), else one, since every part is written and read once more (32 such tokens,
+    // 8000 cells: 33 us, with two 41; 1 token, 16000 cells: 23 and 25), and 256 cells and more in each (24 tokens of 32 heads, 2047 cells: 18 us, with 128 cells 23).  Of a token's own cells four waves' worth of what is left of two
+    // workgroups a compute unit, 16 words of the mask and more each
     A.prompt_parts = A.own_parts = 0;
     A.prompt_share = A.own_share = 1;
     if (A.prompt > 0) {
-        A.prompt_share = px_share_of(A.prompt, 32, (int) std::max<int64_t>(1, std::min<int64_t>(target / units, (A.prompt + 255) / 256)));
+        const int64_t two = std::min<int64_t>(PX_PARTS - 64, target / units), most = A.prompt / std::max<int64_t>(1, two) >= 1024 ? two : target / 2 / units;
+        A.prompt_share = px_share_of(A.prompt, 32, (int) std::max<int64_t>(1, std::min<int64_t>(most, (A.prompt + 255) / 256)));
         A.prompt_parts = (A.prompt + A.prompt_share - 1) / A.prompt_share;
     }
     if (A.n_kv > A.prompt) {
         const int64_t left = std::max<int64_t>(4 * (target - A.prompt_parts * units), own);          // (waves of workgroups that run beside the prompt's)
-        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(left / own, (words + 15) / 16)));
+        const int64_t most = std::min<int64_t>(left / own, PX_PARTS - A.prompt_parts);
+        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(most, (words + 15) / 16)));
         A.own_parts = (words + A.own_share - 1) / A.own_share;
     }
     A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_row_blocks = px_divide_by(std::max(1, A.row_blocks)); A.by_own_blocks = px_divide_by(A.own_blocks); A.by_own_parts = px_divide_by(std::max(1, A.own_parts));
+    A.by_parts = px_divide_by(std::max(1, A.prompt_parts + A.own_parts)); A.by_quads = px_divide_by(A.dim / 4);
 }
 
 static int px_sizes(const char * what, int dim, int heads, int kv, int n_tok, int prompt, int n_kv) {
@@ -476,9 +492,9 @@ template <int DP> static int px_launch(const px_args & A, hipStream_t s) {
     }
     if (parts != 1) {
         const int at_once = 256 / (A.dim / 4);
-        int groups = 1;
-        while (groups * 4 < parts && groups * 2 <= at_once) groups *= 2;
-        const int here = at_once / groups;
+        int groups = 0;                                      // (as a power of two)
+        while (4 << groups < parts && 2 << groups <= at_once) groups++;
+        const int here = at_once >> groups;
         const int64_t grid = ((int64_t) A.n_tok * A.heads + here - 1) / here;
         PI_KT_LAUNCH(PI_KT_ATT, 0, nta, 4.0 * A.n_tok * A.heads * ((double) parts * (A.dim + 2) + A.dim), k_prefix_merge, dim3((unsigned) grid), dim3(256), 0, s, A, parts, groups, here, pi_abort_word());
         PI_CHECK_LAUNCH();

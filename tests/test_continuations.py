@@ -173,6 +173,23 @@ def test_attention(heads, kv, dim, tokens, prompt, own):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prompt,own", [(0, 1 << 20), (1 << 20, 0), (600000, 500000)])
+def test_a_million_cells_of_one_head(prompt, own):
+    """as many parts of a row as there can be; the values are positive, so that an output's error is the weights'"""
+    U, lib = gpu()
+    rng = np.random.default_rng(own + 1)
+    q, k, _, seen = inputs(rng, 1, 1, 8, 1, prompt, own, loners=False)
+    k = np.nan_to_num(k)
+    v = (0.5 + rng.random(k.shape)).astype(np.float16)
+    seen[:] = True
+    p = Pass(U, lib, q, k, v, seen, prompt, 8 ** -0.5)
+    p.attend()
+    got, lse = p.outputs()
+    want, want_lse, _ = soft_max(q, k, v, seen, 8 ** -0.5)
+    check_attention(got, want, lse, want_lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(32, 4, 64, 4, 500, 40), (8, 2, 128, 50, 300, 100)])
 def test_sizes_on_the_device(heads, kv, dim, tokens, prompt, own):
     """room for more cells than there are: the device says how many are shared and live; parts without a cell count for nothing, and the mass of what is not live stays"""
