@@ -636,14 +636,16 @@ template <bool WIDE, int STEPS> static __device__ __forceinline__ void sp_slice_
 
 template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
-    __shared__ uint32_t bins[SP_COARSE], bounds[4];
+    __shared__ uint32_t bins[SP_COARSE], bounds[4], whole[4];
     __shared__ sp_u64 tops[4];
     __shared__ float firsts[4];
     __shared__ double overs[4];
     __shared__ int listed;
     __shared__ double table[SP_TABLE];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, base = slice * SP_SLICE + wave * (SP_SLICE / 4);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     sp_row R(A, row, table);
+    // (the row's last values for the last slice, so that its waves are as full as the others': the fewer lanes, the lower a bound.  What stands in the slice before is taken out once the bound is known)
+    const int begin = slice * SP_SLICE, from = min(begin, R.V - SP_SLICE), base = from + wave * (SP_SLICE / 4);
     float x[32], first = -INFINITY;
     sp_slice_load<WIDE, 8>(R, base, x);
     const bool few = R.k > 0 && R.k <= 128, border = !few && (R.k > 0 || R.nucleus());
@@ -656,11 +658,22 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     float mine = -INFINITY; int mine_id = 0;
 #pragma unroll
     for (int e = 0; e < 32; e++) if (x[e] > mine) { mine = x[e]; mine_id = sp_slice_id<WIDE>(base, e / 4, e % 4); }
+    auto own_ones = [&]() __attribute__((always_inline)) {
+        if (from == begin) return;
+#pragma unroll
+        for (int e = 0; e < 32; e++) if (sp_slice_id<WIDE>(base, e / 4, e % 4) < begin) x[e] = -INFINITY;
+    };
     if (few) {
-        const uint32_t b = sp_bound(sp_key(mine), (R.k + 3) / 4);
+        // (of the waves whose lanes all have something, each its share of k; without one there is little to list)
+        const bool full = __all(mine > -INFINITY);
+        if (lane == 0) whole[wave] = full;
+        __syncthreads();
+        const int waves = (int) (whole[0] + whole[1] + whole[2] + whole[3]);
+        const uint32_t b = full ? sp_bound(sp_key(mine), (R.k + waves - 1) / waves) : waves > 0 ? ~0u : 0u;
         if (lane == 0) bounds[wave] = b;
         __syncthreads();
         const float least = sp_at_least(min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3])));
+        own_ones();
         sp_u64 * list = S.lists + ((int64_t) row * slices + slice) * SP_SLICE_LIST;
 #pragma unroll
         for (int e = 0; e < 32; e++) {
@@ -675,6 +688,7 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
         if (tid == 0) mine_of->listed = (sp_u64) listed;
         return;
     }
+    own_ones();
     sp_u64 top = sp_wave_top(mine > -INFINITY ? sp_rank(mine, mine_id) : 0);
     first = pi_wave_max(first);
     if (lane == 0) { tops[wave] = top; firsts[wave] = first; }

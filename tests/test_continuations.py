@@ -381,6 +381,25 @@ def test_sample(vocab, stride):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [32769, 33000, 40960, 40961, 50000, 250000, 524287, 524288])
+def test_sample_of_the_few_best(vocab):
+    """rows whose last part is short, the best in front, behind and where parts meet, allowed ids in one place, fewer than are asked for"""
+    U, lib = gpu()
+    rng = np.random.default_rng(vocab)
+    x = (2.5 * rng.standard_normal((8, vocab))).astype(np.float32)
+    x[1, :vocab - 300] = -np.inf
+    x[2, :8000] = x[2, 8400:] = -np.inf
+    x[3, vocab - 8300:vocab - 8100] += 20
+    x[4] = -np.inf; x[4, rng.integers(0, vocab, 5)] = 1.0
+    x[5, -1] = x[5, 0] = x[5, 8191] = x[5, 8192] = x[5].max() + 1
+    x[6, rng.random(vocab) < 0.97] = -np.inf
+    x[7, vocab // 8192 * 8192 - 60:][:120] += 15
+    for k in (1, 2, 20, 100, 128):
+        check_sample(U, lib, x, vocab, (np.full(8, 0.8), np.full(8, k), None, None), rng.random(8))
+    check_sample(U, lib, x, vocab, (np.full(8, 1.1), np.full(8, 64), np.full(8, 0.9), np.full(8, 0.01)), rng.random(8))
+
+
+@pytest.mark.gpu
 def test_sample_of_odd_rows():
     """rows of equal logits (the border inside them goes by the id), of few values, of nothing, with infinities and what is no number, one logit far above; the ends of u"""
     U, lib = gpu()
