@@ -306,6 +306,24 @@ static __device__ __forceinline__ uint32_t sp_bound(uint32_t key, int r) {
     return t;
 }
 static __device__ __forceinline__ uint32_t sp_key(float v) { return v > -INFINITY ? (uint32_t) (sp_rank(v, 0) >> 32) : 0u; }
+// The waves with a value, `mine` the largest, in enough of their lanes for twice their share of the first k (and in a quarter of them) bound it: each a share of all k; without one there is little to list.  (A wave with few has a
+// low bound: where all took part, a row of 31000 whose last wave had 280 values took 26 us, one of 32000 12; where only those with something in every lane did, 4 masked rows of 8000 took 20 instead of 9)
+template <int WAVES> static __device__ __forceinline__ uint32_t sp_wave_bound(uint32_t * bounds, float mine, int k) {
+    const int wave = threadIdx.x >> 6, have = __popcll(__ballot(mine > -INFINITY));
+    const bool joins = have >= max(16, 2 * ((k + WAVES - 1) / WAVES));
+    if ((threadIdx.x & 63) == 0) bounds[WAVES + wave] = joins;
+    __syncthreads();
+    uint32_t waves = 0, bound = ~0u;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) waves += bounds[WAVES + i];
+    if (waves == 0) return 0;
+    const uint32_t b = joins ? sp_bound(sp_key(mine), (k + (int) waves - 1) / (int) waves) : ~0u;
+    if ((threadIdx.x & 63) == 0) bounds[wave] = b;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) bound = min(bound, bounds[i]);
+    return bound;
+}
 static __device__ __forceinline__ float sp_at_least(uint32_t key) { return key == 0 ? -INFINITY : sp_value((sp_u64) key << 32); }
 
 // The first k of the order are among the n <= 128 of L.list: the rest of the way by one wave.  A lane has the places `lane` and, where there are more than 64, lane + 64 of the order
@@ -426,26 +444,26 @@ static __device__ __forceinline__ void sp_of_best(const sp_args & A, sp_row & R,
 
 // A row by one workgroup.  VPT > 0: up to 1024 VPT values stay in registers.  A wave has a run of `chunk` ids, 256 of them a step: four to a lane side by side where rows lie on 16 bytes and end there (WIDE)
 template <int VPT, bool WIDE> struct sp_values {
-    const float * x; int V, steps, chunk, first, lane;
+    const float * x; int V, steps, chunk, first, end, lane;
     float own[VPT > 0 ? VPT : 1];
     __device__ __forceinline__ int id(int j, int e) const { return first + 256 * j + (WIDE ? 4 * lane + e : 64 * e + lane); }
     // (without a branch, so that many are on their way at once)
     __device__ __forceinline__ void load(int j, float * to, int at) const {
         if constexpr (WIDE) {
             const float4 v = *(const float4 *) (x + min(id(j, 0), V - 4));
-            const bool is = j < steps && id(j, 0) < V;
+            const bool is = j < steps && id(j, 0) < end;
             to[at] = is ? v.x : -INFINITY; to[at + 1] = is ? v.y : -INFINITY; to[at + 2] = is ? v.z : -INFINITY; to[at + 3] = is ? v.w : -INFINITY;
         } else
 #pragma unroll
-            for (int e = 0; e < 4; e++) { const float v = x[min(id(j, e), V - 1)]; to[at + e] = j < steps && id(j, e) < V ? v : -INFINITY; }
+            for (int e = 0; e < 4; e++) { const float v = x[min(id(j, e), V - 1)]; to[at + e] = j < steps && id(j, e) < end ? v : -INFINITY; }
     }
     __device__ __forceinline__ sp_values(const float * row, int n) : x(row), V(n) {
-        lane = threadIdx.x & 63; steps = (V + 256 * SP_WAVES - 1) / (256 * SP_WAVES); chunk = 256 * steps; first = (int) (threadIdx.x >> 6) * chunk;
+        lane = threadIdx.x & 63; chunk = (V + 4 * SP_WAVES - 1) / (4 * SP_WAVES) * 4; steps = (chunk + 255) / 256; first = (int) (threadIdx.x >> 6) * chunk; end = min(first + chunk, V);
         if constexpr (VPT > 0)
 #pragma unroll
             for (int j = 0; j < VPT / 4; j++) load(j, own, 4 * j);
     }
-    // f(value, id) of the thread's values, minus infinity for what is not there (whole waves call)
+    // f(value, id) of the thread's values, minus infinity for what is not there or another wave's (whole waves call)
     template <class F> __device__ __forceinline__ void every(F && f) const {
         if constexpr (VPT > 0) {
 #pragma unroll
@@ -576,6 +594,7 @@ template <class S> static __device__ __forceinline__ void sp_any_number(const sp
 template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sample(const sp_args A, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w);
     __shared__ sp_shared L;
+    __shared__ uint32_t bounds[2 * SP_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
     sp_row R(A, row, L.table);
     const sp_values<VPT, WIDE> X(R.x, R.V);
@@ -587,13 +606,7 @@ template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sa
     const bool few = R.k > 0 && R.k <= 128;
     sp_u64 top = 0;
     if (few) {                                               // (the largest comes with the list)
-        const uint32_t b = sp_bound(sp_key(mine), (R.k + SP_WAVES - 1) / SP_WAVES);
-        if (lane == 0) L.count[wave] = b;
-        __syncthreads();
-        uint32_t bound = L.count[0];
-#pragma unroll
-        for (int i = 1; i < SP_WAVES; i++) bound = min(bound, L.count[i]);
-        const float least = sp_at_least(bound);
+        const float least = sp_at_least(sp_wave_bound<SP_WAVES>(bounds, mine, R.k));
         const int n = sp_gather(X, L, [&](float v, int) __attribute__((always_inline)) { return v >= least; });
         if (n == 0) {
             if (tid == 0) sp_leave(A, row, -1, 0.0f, 0);
@@ -636,7 +649,7 @@ template <bool WIDE, int STEPS> static __device__ __forceinline__ void sp_slice_
 
 template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
-    __shared__ uint32_t bins[SP_COARSE], bounds[4], whole[4];
+    __shared__ uint32_t bins[SP_COARSE], bounds[8];
     __shared__ sp_u64 tops[4];
     __shared__ float firsts[4];
     __shared__ double overs[4];
@@ -664,15 +677,7 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
         for (int e = 0; e < 32; e++) if (sp_slice_id<WIDE>(base, e / 4, e % 4) < begin) x[e] = -INFINITY;
     };
     if (few) {
-        // (of the waves whose lanes all have something, each its share of k; without one there is little to list)
-        const bool full = __all(mine > -INFINITY);
-        if (lane == 0) whole[wave] = full;
-        __syncthreads();
-        const int waves = (int) (whole[0] + whole[1] + whole[2] + whole[3]);
-        const uint32_t b = full ? sp_bound(sp_key(mine), (R.k + waves - 1) / waves) : waves > 0 ? ~0u : 0u;
-        if (lane == 0) bounds[wave] = b;
-        __syncthreads();
-        const float least = sp_at_least(min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3])));
+        const float least = sp_at_least(sp_wave_bound<4>(bounds, mine, R.k));
         own_ones();
         sp_u64 * list = S.lists + ((int64_t) row * slices + slice) * SP_SLICE_LIST;
 #pragma unroll

@@ -381,7 +381,7 @@ def test_sample(vocab, stride):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("vocab", [32769, 33000, 40960, 40961, 50000, 250000, 524287, 524288])
+@pytest.mark.parametrize("vocab", [8400, 9000, 16500, 20001, 31000, 32769, 33000, 40960, 40961, 50000, 250000, 524287, 524288])
 def test_sample_of_the_few_best(vocab):
     """rows whose last part is short, the best in front, behind and where parts meet, allowed ids in one place, fewer than are asked for"""
     U, lib = gpu()
