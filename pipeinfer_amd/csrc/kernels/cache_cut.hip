@@ -13,11 +13,11 @@
 #define CC_KEYS 28672        /* keys in LDS (112 KB); cells that move, as many at a time */
 #define CC_CELLS 131072      /* cells of the bitmap */
 
-// order of the cells: guarded, then by mass (-0 like 0), what is no number last
+// order of the cells: guarded, then by mass (-0 like 0), what is no number last; 0 is no cell's
 static __device__ __forceinline__ uint32_t cc_key(float x, bool guarded) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     const uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return guarded ? 0xffffffffu : x != x ? 0u : k;
+    return guarded ? 0xffffffffu : x != x ? 1u : k;
 }
 
 // the sum over the workgroup's threads ahead of this one, and over all of them (sixteen waves; two barriers)
@@ -33,8 +33,8 @@ static __device__ __forceinline__ uint32_t cc_before(uint32_t v, uint32_t * wave
 }
 
 // One workgroup.  The boundary's key: its first 11 bits from the counts of all keys, the rest by digits of 11 and 10 bits of those that share them, listed in LDS (of all keys where the list does not hold them).  What stays is then a bit of
-// a bitmap in LDS, and where a cell goes follows from the bits ahead of it: no pass walks the cells in their order.  Bound by the instructions of one compute unit, a handful per pass and 64 cells: keys of up to CC_KEYS cells stay in LDS,
-// the others' are made again from the masses.
+// a bitmap in LDS, and where a cell goes follows from the bits ahead of it: no pass walks the cells in their order.  Bound by the instructions of one compute unit, a handful per pass and 64 cells: keys of CC_KEYS cells stay in LDS, of
+// 4096 more in registers, the others' are made again from the masses.  (32768 cells: 25 us, 19 of them the keys, their counts and the passes over them; with loops over cells, tests in every lane, 31.)
 struct cc_shared {
     __attribute__((aligned(16))) uint32_t bins[CC_BINS], words[2 * CC_CELLS / 32], waves[CC_THREADS / 64], found[4];
     __attribute__((aligned(16))) uint32_t keys[CC_KEYS];       // then the cells that move
@@ -51,29 +51,55 @@ __global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __res
         if (__all(in && bin == b0)) { if (lane == 0) atomicAdd(&L.bins[b0], 64u); }              // (equal masses: one address)
         else if (in) atomicAdd(&L.bins[bin], 1u);
     };
-    // the keys, eight cells a thread on their way at a time
-    for (int c0 = 0; c0 < cells; c0 += 8 * CC_THREADS) {
+    // the keys, eight cells a thread on their way at a time; in LDS zeros behind the last of them, to the end of a round of four steps
+    const int steps = (cells + CC_THREADS - 1) / CC_THREADS;
+    constexpr int HELD = CC_KEYS / CC_THREADS;
+    uint32_t behind[4] = {};                                   // the four steps behind those in LDS
+    for (int i0 = 0; i0 < steps; i0 += 8) {
         float m[8]; uint32_t g[8] = {};
 #pragma unroll
-        for (int j = 0; j < 8; j++) m[j] = mass[min(c0 + j * CC_THREADS + tid, cells - 1)];
+        for (int j = 0; j < 8; j++) m[j] = mass[min((i0 + j) * CC_THREADS + tid, cells - 1)];
         if (guard)
 #pragma unroll
-            for (int j = 0; j < 8; j++) g[j] = guard[min(c0 + j * CC_THREADS + tid, cells - 1) >> 5];
+            for (int j = 0; j < 8; j++) g[j] = guard[min((i0 + j) * CC_THREADS + tid, cells - 1) >> 5];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int c = c0 + j * CC_THREADS + tid;
-            if (c - lane >= cells) break;
-            const uint32_t key = cc_key(m[j], g[j] >> (tid & 31) & 1);
-            if (c < CC_KEYS) L.keys[c] = key;
-            count(c < cells, key >> 21);
+            const int c = (i0 + j) * CC_THREADS + tid;
+            if (i0 + j >= (steps + 3 & ~3)) break;
+            const uint32_t key = c < cells ? cc_key(m[j], g[j] >> (tid & 31) & 1) : 0u;
+            if (i0 + j < HELD) L.keys[c] = key;
+            if (j >= HELD % 8 && j < HELD % 8 + 4 && i0 == HELD / 8 * 8) behind[j & 3] = key;
+            if (i0 + j < steps) count(key != 0, key >> 21);
         }
     }
-    // f(cell, is one, key) for every CC_THREADS-th cell, whole waves at a time
+    // f(step, key) for every CC_THREADS-th cell, four keys on their way; 0 where there is no cell
     auto each = [&](auto && f) __attribute__((always_inline)) {
-        const int held = min(cells, CC_KEYS);
-        int c = tid;
-        for (; c - lane < held; c += CC_THREADS) f(c, c < cells, L.keys[min(c, CC_KEYS - 1)]);
-        for (; c - lane < cells; c += CC_THREADS) f(c, c < cells, c < cells ? cc_key(mass[c], guard && (guard[c >> 5] >> (c & 31) & 1)) : 0u);
+        static_assert(HELD % 4 == 0 && CC_CELLS % (32 * CC_THREADS) == 0, "");
+        int i = 0;
+#pragma unroll 1
+        for (; i < min(steps, HELD); i += 4) {
+            uint32_t key[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) key[j] = L.keys[(i + j) * CC_THREADS + tid];
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(i + j, key[j]);
+        }
+        if (i < steps) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(i + j, behind[j]);
+            i += 4;
+        }
+#pragma unroll 1
+        for (; i < steps; i += 4) {                          // (from memory, where one at a time is a microsecond a step)
+            float m[4]; uint32_t g[4] = {};
+#pragma unroll
+            for (int j = 0; j < 4; j++) m[j] = mass[min((i + j) * CC_THREADS + tid, cells - 1)];
+            if (guard)
+#pragma unroll
+                for (int j = 0; j < 4; j++) g[j] = guard[min((i + j) * CC_THREADS + tid, cells - 1) >> 5];
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(i + j, (i + j) * CC_THREADS + tid < cells ? cc_key(m[j], g[j] >> (tid & 31) & 1) : 0u);
+        }
     };
     uint32_t prefix = 0, left = (uint32_t) keep, same = 0;     // of the `same` cells whose key begins like `prefix` `left` stay, the lowest; all above stay, none below
     // from the top bin down, two to a thread
@@ -97,10 +123,11 @@ __global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __res
     const uint32_t in_list = same;
     if (same != left && listed) {
         uint32_t mine = 0;                                   // (counted first: no store waits for an atomic)
-        each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { mine += is && key >> 21 == prefix; });
+        const uint32_t least = max(prefix << 21, 1u), span = ((prefix + 1) << 21) - least;
+        each([&](int, uint32_t key) __attribute__((always_inline)) { mine += key - least < span; });
         if (__any(mine > 0)) {
             uint32_t at = mine > 0 ? atomicAdd(&L.found[3], mine) : 0;
-            each([&](int, bool is, uint32_t key) __attribute__((always_inline)) { if (is && key >> 21 == prefix) list[at++] = key; });
+            each([&](int, uint32_t key) __attribute__((always_inline)) { if (key - least < span) list[at++] = key; });
         }
         __syncthreads();
     }
@@ -108,25 +135,35 @@ __global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __res
         const int width = 11 - pass, from = shift - width;
         for (int i = tid; i < CC_BINS; i += CC_THREADS) L.bins[i] = 0;
         __syncthreads();
-        auto digit = [&](int, bool is, uint32_t key) __attribute__((always_inline)) { count(is && key >> shift == prefix, key >> from & ((1u << width) - 1)); };
-        if (listed) for (uint32_t i = tid; i - lane < in_list; i += CC_THREADS) digit(0, i < in_list, list[min(i, in_list - 1)]);
+        auto digit = [&](int, uint32_t key) __attribute__((always_inline)) { count(key != 0 && key >> shift == prefix, key >> from & ((1u << width) - 1)); };
+        if (listed) for (uint32_t i = tid; i - lane < in_list; i += CC_THREADS) digit(0, i < in_list ? list[i] : 0u);
         else each(digit);
         border(width);
         shift = from;
     }
     __syncthreads();
     // the bitmap of what stays; where not all of the boundary's key do, the first of them
-    const uint32_t bound = prefix << shift;
-    const bool some = same != left;
+    const uint32_t bound = max(prefix << shift, 1u);
+    const bool some = same != left;                            // (then `bound` is the boundary's whole key)
     const int words = (cells + 31) / 32;
-    each([&](int c, bool is, uint32_t key) __attribute__((always_inline)) {
-        const unsigned long long who = __ballot(is && key >= bound);
-        if (lane == 0) *(unsigned long long *) (bitmap + c / 32) = who;          // (a step past the end writes zeros)
+    uint32_t stay = 0, equal = 0;                              // lane l: half l & 1 of step l / 2, of 32 steps
+    auto leave = [&](int step) __attribute__((always_inline)) {
+        const int at = ((step & ~31) + lane / 2) * (CC_THREADS / 32) + 2 * wave + (lane & 1);
+        bitmap[at] = stay;
+        if (some) ahead[at] = equal;
+        stay = equal = 0;
+    };
+    each([&](int i, uint32_t key) __attribute__((always_inline)) {
+        const bool mine = lane >> 1 == (i & 31);
+        const unsigned long long who = __ballot(key >= bound);
+        stay = mine ? lane & 1 ? (uint32_t) (who >> 32) : (uint32_t) who : stay;
         if (some) {
-            const unsigned long long eq = __ballot(is && key >> shift == prefix);
-            if (lane == 0) *(unsigned long long *) (ahead + c / 32) = eq;
+            const unsigned long long eq = __ballot(key == bound);
+            equal = mine ? lane & 1 ? (uint32_t) (eq >> 32) : (uint32_t) eq : equal;
         }
+        if ((i & 31) == 31) leave(i);
     });
+    if ((steps + 3 & ~3) & 31) leave(steps - 1);
     __syncthreads();
     uint32_t all;
     if (some) {
@@ -159,18 +196,33 @@ __global__ void __launch_bounds__(CC_THREADS) k_cache_choose(const float * __res
         if (part == 0) edge_free = L.found[0];
     }
     for (uint32_t w0 = 0; w0 == 0 || w0 < total; w0 += CC_KEYS) {
-        for (int c = (int) edge * 32 + tid; c < cells; c += CC_THREADS) {
-            const uint32_t w = (uint32_t) c / 32, b = w == edge ? bitmap[w] & ~in_front : bitmap[w];
-            if (!(b >> (c & 31) & 1)) continue;
-            const uint32_t r = (w == edge ? 0 : ahead[w]) + (uint32_t) __popc(b & ((1u << (c & 31)) - 1)) - w0;
-            if (r < CC_KEYS) L.keys[r] = (uint32_t) c;           // (r wraps far above for those of earlier windows)
+#pragma unroll 1
+        for (int i = keep / (4 * CC_THREADS) * 4; i < steps; i += 4) {
+            uint32_t b[4], r[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const int w = (i + j) * (CC_THREADS / 32) + tid / 32; b[j] = bitmap[w]; r[j] = ahead[w]; }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = (i + j) * CC_THREADS + tid;
+                if ((uint32_t) c / 32 == edge) { b[j] &= ~in_front; r[j] = 0; }
+                r[j] += (uint32_t) __popc(b[j] & ((1u << (tid & 31)) - 1)) - w0;               // (wraps far above for those of earlier windows)
+                if (c >= keep && (b[j] >> (tid & 31) & 1) && r[j] < CC_KEYS) L.keys[r[j]] = (uint32_t) c;
+            }
         }
         __syncthreads();
-        for (int c = tid; c < keep; c += CC_THREADS) {
-            const uint32_t w = (uint32_t) c / 32, b = bitmap[w];
-            if (b >> (c & 31) & 1) { if (w0 == 0) source[c] = c; continue; }
-            const uint32_t r = (w == edge ? edge_free : ahead[w]) + (uint32_t) __popc(~b & ((1u << (c & 31)) - 1)) - w0;
-            if (r < CC_KEYS) source[c] = (int32_t) L.keys[r];
+#pragma unroll 1
+        for (int i = 0; i * CC_THREADS < keep; i += 4) {
+            uint32_t b[4], r[4], k[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) { const int w = (i + j) * (CC_THREADS / 32) + tid / 32; b[j] = bitmap[w]; r[j] = (uint32_t) w == edge ? edge_free : ahead[w]; }
+#pragma unroll
+            for (int j = 0; j < 4; j++) { r[j] += (uint32_t) __popc(~b[j] & ((1u << (tid & 31)) - 1)) - w0; k[j] = L.keys[min(r[j], (uint32_t) CC_KEYS - 1)]; }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = (i + j) * CC_THREADS + tid;
+                const bool stays = b[j] >> (tid & 31) & 1;
+                if (c < keep && (stays ? w0 == 0 : r[j] < CC_KEYS)) source[c] = stays ? c : (int32_t) k[j];
+            }
         }
         __syncthreads();
     }
