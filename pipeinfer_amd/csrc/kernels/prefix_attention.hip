@@ -128,7 +128,7 @@ struct px_args {
     int dim, heads, kv, group, n_tok, prompt, n_kv;
     int row_blocks, prompt_parts, own_blocks, own_parts;     // of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
     px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts, by_parts, by_quads;
-    int prompt_share, own_share;                             // cells, words of the mask of a part where the sizes are the arguments'
+    int prompt_share, own_share; bool together;                             // cells, words of the mask of a part where the sizes are the arguments'
     float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
     float * out; int64_t out_stride; float * lse;
 };
@@ -321,41 +321,52 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
     px_u32x4 q[DP / 16];
     px_sums<DP> S;
     uint8_t * mine = lds + wave * 32 * px_lds<DP>::V;
-    if (blockIdx.x < prompt_blocks) {
+    const bool shared = blockIdx.x < prompt_blocks;
+    int part, kvh, tok, head, in, rows = A.group;              // in: the lane's row, of `rows`
+    uint32_t whose = 0;                                        // (the token whose own cells are walked)
+    if (shared) {
         // the blocks of rows that read the same keys follow each other on one XCD (a workgroup's is its number modulo 8)
         const uint32_t b = blockIdx.x, eights = pairs % 8 == 0, of = eights ? b >> 3 : b, by = px_quotient(of, A.by_row_blocks), block = of - by * A.row_blocks, pair = eights ? by * 8 + (b & 7) : by;
-        const uint32_t part = px_quotient(pair, A.by_kv), kvh = pair - part * A.kv;
+        part = (int) px_quotient(pair, A.by_kv); kvh = (int) pair - part * A.kv;
         int c0, c1;
-        px_share(prompt, A.dyn ? px_share_of(prompt, 32, A.prompt_parts) : A.prompt_share, (int) part, c0, c1);
-        const int rows = A.n_tok * A.group;
+        px_share(prompt, A.dyn ? px_share_of(prompt, 32, A.prompt_parts) : A.prompt_share, part, c0, c1);
+        rows = A.n_tok * A.group;
         if constexpr (WIDE) {
             if (c0 >= c1) {                                  // (fewer cells than there may be)
                 px_start(S);
-                const int row = block * 128 + wave * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group);
-                px_leave<DP>(A, S, (int) part, tok, (int) kvh * A.group + at - tok * A.group, row < rows, g);
-            } else px_wide<DP>(A, lds, (int) kvh, (int) block, (int) part, c0, c1);
+                in = block * 128 + wave * 32 + n;
+                const int at = min(in, rows - 1);
+                tok = (int) px_quotient((uint32_t) at, A.by_group);
+                px_leave<DP>(A, S, part, tok, kvh * A.group + at - tok * A.group, in < rows, g);
+            } else px_wide<DP>(A, lds, kvh, (int) block, part, c0, c1);
+            return;
         } else {
-            const int row = block * 32 + n, at = min(row, rows - 1), tok = (int) px_quotient((uint32_t) at, A.by_group), head = (int) kvh * A.group + at - tok * A.group;
+            in = block * 32 + n;
+            const int at = min(in, rows - 1);
+            tok = (int) px_quotient((uint32_t) at, A.by_group); head = kvh * A.group + at - tok * A.group;
             px_queries<DP>(A, q, tok, head, g);
             px_start(S);
-            px_walk<DP>(A, S, q, mine, (int) kvh, 32 * wave, 128, lane, c1 - c0, [&](int i) __attribute__((always_inline)) { return c0 + i; });
-            px_meet<DP>(A, S, lds, wave, lane, (int) part, tok, head, row < rows);
+            px_walk<DP>(A, S, q, mine, kvh, 32 * wave, 128, lane, c1 - c0, [&](int i) __attribute__((always_inline)) { return c0 + i; });
         }
-        return;
     }
-    // a token's own cells: a wave takes 32 of the query heads of one key head, and 64 words of the mask at a time
-    const uint32_t unit = (blockIdx.x - prompt_blocks) * 4 + __builtin_amdgcn_readfirstlane(wave);
-    const uint32_t a = px_quotient(unit, A.by_kv), kvh = unit - a * A.kv, c = px_quotient(a, A.by_own_blocks), block = a - c * A.own_blocks, tok = px_quotient(c, A.by_own_parts), part = c - tok * A.own_parts;
-    if (tok >= (uint32_t) A.n_tok) return;
-    const int in = (int) block * 32 + n, head = (int) kvh * A.group + min(in, A.group - 1), words = (A.n_kv + 31) / 32, w0 = prompt / 32, w_all = max(0, (n_kv + 31) / 32 - w0);
+    // A token's own cells: a wave takes 32 of the query heads of one key head, and 64 words of the mask at a time; or, of a single token behind a short prompt, the four waves of the prompt's workgroup, every fourth 32 cells each
+    const int words = (A.n_kv + 31) / 32, w0 = prompt / 32, w_all = max(0, (n_kv + 31) / 32 - w0);
     uint16_t * list = (uint16_t *) (lds + 4 * 32 * px_lds<DP>::V) + wave * PX_LIST;
-    int from, to;
-    px_share(w_all, A.dyn ? px_share_of(w_all, 8, A.own_parts) : A.own_share, (int) part, from, to);
-    px_queries<DP>(A, q, (int) tok, head, g);
-    px_start(S);
+    int from = 0, to = A.together ? w_all : 0;
+    if (!shared) {
+        const uint32_t unit = (blockIdx.x - prompt_blocks) * 4 + __builtin_amdgcn_readfirstlane(wave);
+        const uint32_t a = px_quotient(unit, A.by_kv), c = px_quotient(a, A.by_own_blocks);
+        whose = px_quotient(c, A.by_own_parts);
+        if (whose >= (uint32_t) A.n_tok) return;
+        kvh = (int) (unit - a * A.kv); tok = (int) whose; part = (int) (c - whose * A.own_parts); in = (int) (a - c * A.own_blocks) * 32 + n; head = kvh * A.group + min(in, A.group - 1);
+        px_share(w_all, A.dyn ? px_share_of(w_all, 8, A.own_parts) : A.own_share, part, from, to);
+        part += A.prompt_parts;
+        px_queries<DP>(A, q, tok, head, g);
+        px_start(S);
+    }
     for (int w = from; w < to; w += 64) {
         const int at = w0 + min(w + lane, to - 1);
-        uint32_t bits = A.mask[(int64_t) tok * words + at];
+        uint32_t bits = A.mask[(int64_t) whose * words + at];
         if (w + lane >= to) bits = 0;
         if (32 * at < prompt) bits &= ~0u << (prompt - 32 * at);                // (prompt - 32 * at < 32: at >= prompt / 32)
         if (n_kv - 32 * at < 32) bits &= (1u << (n_kv - 32 * at)) - 1;
@@ -364,10 +375,11 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
         for (uint32_t left = bits; left; left &= left - 1) list[before++] = (uint16_t) (32 * lane + __builtin_ctz(left));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         const int first = 32 * (w0 + w);
-        px_walk<DP>(A, S, q, mine, (int) kvh, 0, 32, lane, count, [&](int i) __attribute__((always_inline)) { return first + list[i]; });
+        px_walk<DP>(A, S, q, mine, kvh, shared ? 32 * wave : 0, shared ? 128 : 32, lane, count, [&](int i) __attribute__((always_inline)) { return first + list[i]; });
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    px_leave<DP>(A, S, A.prompt_parts + (int) part, (int) tok, head, in < A.group, g);
+    if (shared) px_meet<DP>(A, S, lds, wave, lane, part, tok, head, in < rows);
+    else px_leave<DP>(A, S, part, tok, head, in < rows, g);
 }
 
 #define PX_PARTS 1088                                            /* what k_prefix_merge has room for; the prompt takes two of a compute unit's at most */
@@ -450,7 +462,11 @@ static void px_plan(px_args & A) {
         A.prompt_share = px_share_of(A.prompt, 32, (int) std::max<int64_t>(1, std::min<int64_t>(most, (A.prompt + 255) / 256)));
         A.prompt_parts = (A.prompt + A.prompt_share - 1) / A.prompt_share;
     }
-    if (A.n_kv > A.prompt) {
+    // A single token behind a short prompt: both by the same workgroup, with nothing left to merge (32 / 4 heads of 64 values, 500 cells and 13 of its own: 8.2 us, in parts 9.9; of 250 cells 7.2 and 10.0; 64 / 8 heads of 128 values,
+    // 250 cells: 9.5 and 10.9; but 500 cells 11.9 and 11.0, and 8 / 2 heads of 256 values, 500 cells: 22.6 and 15.4)
+    A.together = A.n_tok == 1 && A.group <= 32 && A.prompt > 0 && A.prompt <= 512 && A.prompt * A.dim <= 32768 && A.n_kv > A.prompt && A.n_kv - A.prompt <= 256;
+    if (A.together) { A.prompt_parts = 1; A.prompt_share = A.prompt; }
+    else if (A.n_kv > A.prompt) {
         const int64_t left = std::max<int64_t>(4 * (target - A.prompt_parts * units), own);          // (waves of workgroups that run beside the prompt's)
         const int64_t most = std::min<int64_t>(left / own, PX_PARTS - A.prompt_parts);
         A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(most, (words + 15) / 16)));

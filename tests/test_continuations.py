@@ -212,6 +212,26 @@ def test_sizes_on_the_device(heads, kv, dim, tokens, prompt, own):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim", [(32, 4, 64), (8, 8, 128), (31, 1, 40)])
+def test_one_token_behind_a_short_prompt(heads, kv, dim):
+    """the shared and the own cells by the same workgroup: nothing shared, all own ones, gaps, a mask that leaves none, sizes that the device knows"""
+    U, lib = gpu()
+    rng = np.random.default_rng(heads)
+    for prompt, own, live, density, room in ((250, 200, 200, 0.5, None), (1, 256, 256, 1.0, None), (256, 1, 1, 1.0, None), (100, 33, 33, 0.0, None), (0, 5, 5, 1.0, (250, 400)), (77, 100, 100, 0.3, (250, 400)), (250, 0, 0, 1.0, (250, 400)),
+                                             (0, 300, 300, 0.2, (250, 400)), (0, 0, 0, 1.0, (250, 400))):
+        q, k, v, seen = inputs(rng, heads, kv, dim, 1, prompt, own, loners=False)
+        k, v = np.nan_to_num(k), np.nan_to_num(v, posinf=1.0)
+        seen[:, prompt:] = rng.random((1, own)) < density
+        if room:
+            k, v = (np.concatenate([x, np.full((room[1] - len(x), kv, dim), np.nan, np.float16)]) for x in (k, v))
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5, room)
+        p.attend()
+        got, lse = p.outputs()
+        want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
+        check_attention(got, want, lse, want_lse)
+
+
+@pytest.mark.gpu
 def test_scores_far_apart():
     """scores that grow along the cells by far more than the maximum may lag, that fall, and that are huge: the sums are relative to the right maximum"""
     U, lib = gpu()
