@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(1024) k_cache_move(const cm_arrays A, const in
 }
 
 extern "C" int pi_op_cache_move(void * const * arrays, const int64_t * row_bytes, int n_arrays, const int32_t * source, int keep, int cells, void * stream) {
-    if (n_arrays < 0 || keep < 0 || keep > cells) { pi_set_error("pi_op_cache_move: %d arrays, %d of %d cells", n_arrays, keep, cells); return -1; }
+    if (n_arrays < 0 || keep < 0 || keep > cells || cells > 0x7ffff000) { pi_set_error("pi_op_cache_move: %d arrays, %d of %d cells", n_arrays, keep, cells); return -1; }
     if (n_arrays == 0 || keep == 0 || keep == cells) return 0;
     if (!arrays || !row_bytes || !source) { pi_set_error("pi_op_cache_move: arrays, their rows' bytes or source is NULL"); return -1; }
     for (int i = 0; i < n_arrays; i++) if (!arrays[i] || row_bytes[i] < 1 || row_bytes[i] > 0x7fffffff) { pi_set_error("pi_op_cache_move: array %d is NULL or has rows of %lld bytes", i, (long long) row_bytes[i]); return -1; }

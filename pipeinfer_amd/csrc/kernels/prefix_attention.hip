@@ -128,7 +128,8 @@ struct px_args {
     int dim, heads, kv, group, n_tok, prompt, n_kv;
     int row_blocks, prompt_parts, own_blocks, own_parts;     // of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
     px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts, by_parts, by_quads;
-    int prompt_share, own_share; bool together;                             // cells, words of the mask of a part where the sizes are the arguments'
+    int prompt_share, own_share;                             // cells, words of the mask of a part where the sizes are the arguments'
+    bool together;                                           // the prompt's workgroups take the own cells too
     float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
     float * out; int64_t out_stride; float * lse;
 };
@@ -445,7 +446,8 @@ __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts
 
 // ---- how the work is cut ---------------------------------------------------------------------------------------------------------------------------------------------------------------
 static bool px_wide_rows(int rows) { return rows > 64; }
-static void px_plan(px_args & A) {
+// device: the sizes are the device's, which may leave cells behind the prompt where the arguments leave none
+static void px_plan(px_args & A, bool device) {
     const int rows = A.n_tok * A.group, target = 2 * pi_cu_count();
     const bool wide = px_wide_rows(rows);
     A.row_blocks = wide ? (rows + 127) / 128 : (rows + 31) / 32;
@@ -471,7 +473,7 @@ static void px_plan(px_args & A) {
         const int64_t most = std::min<int64_t>(left / own, PX_PARTS - A.prompt_parts);
         A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(most, (words + 15) / 16)));
         A.own_parts = (words + A.own_share - 1) / A.own_share;
-    }
+    } else if (device && A.prompt > 0) A.own_parts = 1;
     A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_row_blocks = px_divide_by(std::max(1, A.row_blocks)); A.by_own_blocks = px_divide_by(A.own_blocks); A.by_own_parts = px_divide_by(std::max(1, A.own_parts));
     A.by_parts = px_divide_by(std::max(1, A.prompt_parts + A.own_parts)); A.by_quads = px_divide_by(A.dim / 4);
 }
@@ -492,7 +494,7 @@ extern "C" size_t pi_op_prefix_attention_scratch_floats(int head_dim, int n_head
     if (px_sizes("pi_op_prefix_attention_scratch_floats", head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0 || n_tok == 0) return 0;
     px_args A{};
     A.dim = head_dim; A.heads = n_head; A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.prompt = n_prompt; A.n_kv = n_kv;
-    px_plan(A);
+    px_plan(A, true);
     return px_floats(A);
 }
 
@@ -534,7 +536,7 @@ extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, co
     px_args A{};
     A.q = q16; A.q_stride = q_stride; A.k = k_cache; A.v = v_cache; A.row = (int64_t) n_head_kv * head_dim; A.mask = mask; A.dyn = dyn; A.c = scale * 1.44269504f;
     A.dim = head_dim; A.heads = n_head; A.kv = n_head_kv; A.group = n_head / n_head_kv; A.n_tok = n_tok; A.prompt = n_prompt; A.n_kv = n_kv; A.out = out; A.out_stride = out_stride; A.lse = lse;
-    px_plan(A);
+    px_plan(A, dyn && mask);
     const size_t need = px_floats(A);
     if (need > 0 && (!scratch || ((uintptr_t) scratch & 15) || scratch_floats < need)) { pi_set_error("%s: %zu floats of scratch, on 16 bytes, for %zu (pi_op_prefix_attention_scratch_floats)", what, scratch ? scratch_floats : 0, need); return -1; }
     A.parts_o = scratch;
@@ -597,7 +599,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         if (tid < 64) lse[to][tid] = next_lse;
     };
     px_f32x16 sum[2] = { px_zero(), px_zero() };
-    const bool masked = cells0 + 256 > prompt;
+    const bool masked = cells0 + 256 > prompt, own = A.mask && n_kv > prompt;             // (without a mask nobody sees a cell behind the prompt)
     if (r0 < r1) { load(r0); store(0); }
     int cur = 0;
     for (int r = r0; r < r1; r += 64, cur ^= 1) {
@@ -618,7 +620,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
                     if constexpr (with_mask) {
                         bits = 0;
                         if (base < n_kv) {
-                            if (base + 32 > prompt) bits = A.mask[(int64_t) px_quotient((uint32_t) min(r + 32 * v + n, r1 - 1), A.by_group) * words + base / 32];
+                            if (own && base + 32 > prompt) bits = A.mask[(int64_t) px_quotient((uint32_t) min(r + 32 * v + n, r1 - 1), A.by_group) * words + base / 32];
                             if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
                             if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
                         }

@@ -32,6 +32,7 @@ def test_attention_refuses(args, why):
     (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 11, P, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, -1, P, None), b"-1 of 10"), (lambda lib, mass: lib.pi_op_cache_choose(None, None, 10, 4, P, None), b"is NULL"),
     (lambda lib, mass: lib.pi_op_cache_choose(P, None, 10, 4, None, None), b"is NULL"),
     (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, P, 11, 10, None), b"11 of 10"), (lambda lib, mass: lib.pi_op_cache_move(None, None, 1, P, 4, 10, None), b"is NULL"),
+    (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, P, 0x7fffff00, 0x7fffffff, None), b"2147483392 of"),
     (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(0), (C.c_int64 * 1)(16), 1, P, 4, 10, None), b"array 0 is NULL"), (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(0), 1, P, 4, 10, None), b"rows of 0 bytes"),
     (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), 1, None, 4, 10, None), b"is NULL"), (lambda lib, mass: lib.pi_op_cache_move((C.c_void_p * 1)(P), (C.c_int64 * 1)(16), -1, P, 4, 10, None), b"-1 arrays"),
     (lambda lib, mass: lib.pi_op_sample(P, 99, 100, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"99 apart"), (lambda lib, mass: lib.pi_op_sample(P, 100, 0, 1, P, P, P, P, P, P, 1 << 30, P, P, P, None), b"1 .. 524288"),
@@ -229,6 +230,33 @@ def test_one_token_behind_a_short_prompt(heads, kv, dim):
         got, lse = p.outputs()
         want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
         check_attention(got, want, lse, want_lse)
+
+
+@pytest.mark.gpu
+def test_nothing_but_the_prompt_by_the_arguments():
+    """without a mask, the prompt's end inside a word; the device says that less is shared: the mask counts then, and without one nothing behind the prompt is there"""
+    U, lib = gpu()
+    rng = np.random.default_rng(23)
+    for tokens, room in ((1, 300), (3, 300), (40, 777)):
+        for prompt, n in ((room, room), (room - 90, room - 20), (0, 70), (37, 37)):
+            q, k, v, seen = inputs(rng, 8, 2, 64, tokens, prompt, n - prompt)
+            k, v = np.nan_to_num(k), np.nan_to_num(v, posinf=1.0)
+            k, v = (np.concatenate([x, np.zeros((room, 2, 64), np.float16)])[:room] for x in (k, v))
+            for masked in (True, False):
+                sees = seen.copy()
+                if not masked:
+                    sees[:, prompt:] = False
+                p = Pass(U, lib, q, k, v, sees, prompt, 0.125, (room, room))
+                if not masked:
+                    p.mask.ptr = None
+                p.attend()
+                got, lse = p.outputs()
+                want, want_lse, w = soft_max(q, k[:n], v[:n], sees, 0.125)
+                check_attention(got, want, lse, want_lse)
+                mass = U.Dev(np.full(room, 3.0, np.float32))
+                p.give(mass, 1.0)
+                m = mass.get(np.float32)
+                assert (m[n:] == 3.0).all() and np.allclose(m[:n], 3.0 + w.sum((0, 1))[:n], rtol=1e-5, atol=1e-5)
 
 
 @pytest.mark.gpu
