@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 typedef _Float16 px_half8 __attribute__((ext_vector_type(8)));
 typedef __fp16 px_half2 __attribute__((ext_vector_type(2)));
@@ -152,19 +153,30 @@ template <int DP> static __device__ __forceinline__ void px_leave(const px_args 
         if (g == 0) A.parts_ml[at] = make_float2(S.m, l);
         if (l == 0.0f) return;                               // (k_prefix_merge leaves such a part out)
     }
+    auto leave = [&](auto whole) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < DP / 32; j++)
+        for (int j = 0; j < DP / 32; j++)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = 32 * j + px_cell(i, g);
-            if (d < A.dim) *(px_f32x4 *) (o + d) = px_f32x4{ S.acc[j][i] * f, S.acc[j][i + 1] * f, S.acc[j][i + 2] * f, S.acc[j][i + 3] * f };
-        }
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * j + px_cell(i, g);
+                if (whole || d < A.dim) *(px_f32x4 *) (o + d) = px_f32x4{ S.acc[j][i] * f, S.acc[j][i + 1] * f, S.acc[j][i + 2] * f, S.acc[j][i + 3] * f };
+            }
+    };
+    if (A.dim == DP) leave(std::true_type{}); else leave(std::false_type{});
 }
 
+// values d .. d + 7 of a row of `dim`, zeros behind its end (read without a branch: behind one, a load is waited for where the branches meet)
+static __device__ __forceinline__ px_u32x4 px_chunk(const uint16_t * row, int d, int dim) {
+    const px_u32x4 x = *(const px_u32x4 *) (row + (d < dim ? d : 0));
+    px_u32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = d < dim ? x[e] : 0u;
+    return y;
+}
 template <int DP> static __device__ __forceinline__ void px_queries(const px_args & A, px_u32x4 (&q)[DP / 16], int tok, int head, int g) {
     const uint16_t * row = A.q + (int64_t) tok * A.q_stride + (int64_t) head * A.dim;
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) q[i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (row + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+    for (int i = 0; i < DP / 16; i++) q[i] = px_chunk(row, 16 * i + 8 * g, A.dim);
 }
 
 // Many rows: a wave has 32 of the workgroup's 128, all walk the same cells, 32 at a time through a ring of four tiles in LDS.  Three tiles are in work at once, so that the matrix cores and the vector unit are: while the weights of tile t are
@@ -207,9 +219,12 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
         for (int i = 0; i < DP / 16; i++) s = px_mfma(*(const px_u32x4 *) (kt + 32 * i), q[i], s);
         return s;
     };
-    load(0); store(0);
-    if (tiles > 1) { load(1); store(1); }
-    if (tiles > 2) load(2);
+    load(0);
+#pragma unroll 1
+    for (int t = 0; t < 2; t++) {                            // (code that runs once costs more than it does)
+        if (t < tiles) store(t);
+        if (t + 1 < tiles) load(t + 1);
+    }
     __syncthreads();
     px_f32x16 s = scores(0);
     px_weights P;
@@ -576,7 +591,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
     for (int u = 0; u < 2; u++) {
         const uint16_t * k = A.k + (int64_t) min(mine + 32 * u + n, n_kv - 1) * A.row + kvh * A.dim;
 #pragma unroll
-        for (int i = 0; i < DP / 16; i++) key[u][i] = 16 * i + 8 * g < A.dim ? *(const px_u32x4 *) (k + 16 * i + 8 * g) : px_u32x4{ 0, 0, 0, 0 };
+        for (int i = 0; i < DP / 16; i++) key[u][i] = px_chunk(k, 16 * i + 8 * g, A.dim);
     }
     float next_lse = INFINITY;
     auto load = [&](int r) __attribute__((always_inline)) {

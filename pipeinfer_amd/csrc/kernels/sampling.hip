@@ -301,7 +301,7 @@ static __device__ __forceinline__ void sp_sort(sp_u64 * list, int n) {
 // a key that at least r of the wave's lanes reach (0: fewer have one), 16 bits of it
 static __device__ __forceinline__ uint32_t sp_bound(uint32_t key, int r) {
     uint32_t t = 0;
-#pragma unroll
+#pragma unroll 1
     for (int b = 31; b >= 16; b--) { const uint32_t c = t | 1u << b; if (__popcll(__ballot(key >= c)) >= r) t = c; }
     return t;
 }
@@ -333,10 +333,10 @@ static __device__ __forceinline__ void sp_of_few(const sp_args & A, sp_row & R, 
         const sp_u64 a = lane < n ? L.list[lane] : 0, b = lane + 64 < n ? L.list[lane + 64] : 0;
         int at_a = 0, at_b = 0;
         if (n <= 64) {
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 0; i < n; i++) at_a += L.list[i] > a;
         } else
-#pragma unroll 4
+#pragma unroll 8
             for (int i = 0; i < n; i++) { const sp_u64 o = L.list[i]; at_a += o > a; at_b += o > b; }
         if (lane < n) L.chance[at_a] = a;
         if (lane + 64 < n) L.chance[at_b] = b;
@@ -481,6 +481,13 @@ template <int VPT, bool WIDE> struct sp_values {
                     for (int e = 0; e < 4; e++) { const float w = v[4 * j + e]; f(w > -INFINITY ? w : -INFINITY, id(j0 + j, e)); }
             }
     }
+    // a bit for each of the thread's values (in registers) that reaches `least`
+    __device__ __forceinline__ uint32_t reach(float least) const {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) bits |= (own[i] >= least && own[i] > -INFINITY ? 1u : 0u) << i;
+        return bits;
+    }
     // f(value, id) of the thread's values that are there
     template <class F> __device__ __forceinline__ void each(F && f) const {
         if constexpr (VPT > 0) {
@@ -500,6 +507,20 @@ template <int VPT, bool WIDE> struct sp_values {
             }
     }
 };
+// The ranks of the values with a bit into `list`, in any order, while there is room; `count` goes up by how many there are.  A few of a row: what is listed is read once more, and the code is short (with a ballot and the store for each of
+// a thread's 32 values, all of it code that runs once, the list of 40 of 32000 took 8000 clocks)
+template <class F> static __device__ __forceinline__ void sp_list_few(uint32_t bits, int * count, int room, sp_u64 * list, const float * x, F && id_of) {
+    const int lane = threadIdx.x & 63, n = __popc(bits), upto = (int) pi_wave_scan((uint32_t) n), all = __builtin_amdgcn_readlane(upto, 63);
+    if (all == 0) return;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(count, all);
+    at = __builtin_amdgcn_readfirstlane(at) + upto - n;
+#pragma unroll 1
+    for (; bits; bits &= bits - 1, at++) {
+        const int id = id_of(__builtin_ctz(bits));
+        if (at < room) list[at] = sp_rank(x[id], id);
+    }
+}
 // the ranks of what `in` says into L.list, in any order; how many there are (more than the list holds: the list is of no use)
 template <class S, class F> static __device__ __forceinline__ int sp_gather(const S & X, sp_shared & L, F && in) {
     __syncthreads();
@@ -599,6 +620,7 @@ template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sa
     sp_row R(A, row, L.table);
     const sp_values<VPT, WIDE> X(R.x, R.V);
     sp_table(L.table);
+    if (tid == 0) L.n = 0;
     if (pi_aborted_together(gone, abort_w)) return;
     // the largest value, a thread's and everybody's, and a bound that at least k of them reach
     float mine = -INFINITY; int mine_id = 0;
@@ -607,7 +629,9 @@ template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sa
     sp_u64 top = 0;
     if (few) {                                               // (the largest comes with the list)
         const float least = sp_at_least(sp_wave_bound<SP_WAVES>(bounds, mine, R.k));
-        const int n = sp_gather(X, L, [&](float v, int) __attribute__((always_inline)) { return v >= least; });
+        sp_list_few(X.reach(least), &L.n, SP_LIST, L.list, R.x, [&](int i) __attribute__((always_inline)) { return X.id(i / 4, i % 4); });
+        __syncthreads();
+        const int n = L.n;
         if (n == 0) {
             if (tid == 0) sp_leave(A, row, -1, 0.0f, 0);
             return;
@@ -680,15 +704,10 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
         const float least = sp_at_least(sp_wave_bound<4>(bounds, mine, R.k));
         own_ones();
         sp_u64 * list = S.lists + ((int64_t) row * slices + slice) * SP_SLICE_LIST;
+        uint32_t bits = 0;
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-            const unsigned long long who = __ballot(x[e] >= least && x[e] > -INFINITY);
-            if (who == 0) continue;
-            int at = 0;
-            if (lane == __builtin_ctzll(who)) at = atomicAdd(&listed, __popcll(who));
-            at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + sp_rank_in(who);
-            if ((who >> lane & 1) && at < SP_SLICE_LIST) list[at] = sp_rank(x[e], sp_slice_id<WIDE>(base, e / 4, e % 4));
-        }
+        for (int e = 0; e < 32; e++) bits |= (x[e] >= least && x[e] > -INFINITY ? 1u : 0u) << e;
+        sp_list_few(bits, &listed, SP_SLICE_LIST, list, R.x, [&](int e) __attribute__((always_inline)) { return sp_slice_id<WIDE>(base, e / 4, e % 4); });
         __syncthreads();
         if (tid == 0) mine_of->listed = (sp_u64) listed;
         return;
