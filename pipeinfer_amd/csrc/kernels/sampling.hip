@@ -463,30 +463,23 @@ template <int VPT, bool WIDE> struct sp_values {
 #pragma unroll
             for (int j = 0; j < VPT / 4; j++) load(j, own, 4 * j);
     }
-    // f(value, id) of the thread's values, minus infinity for what is not there or another wave's (whole waves call)
-    template <class F> __device__ __forceinline__ void every(F && f) const {
+    // in(value, id) of the thread's values as bits (minus infinity for what is not there or another wave's), 32 at a time: done(bits, the first one's step); whole waves call
+    template <class F, class G> __device__ __forceinline__ void marked(F && in, G && done) const {
         if constexpr (VPT > 0) {
+            uint32_t bits = 0;
 #pragma unroll
-            for (int j = 0; j < VPT / 4; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) { const float v = own[4 * j + e]; f(v > -INFINITY ? v : -INFINITY, id(j, e)); }
+            for (int i = 0; i < VPT; i++) bits |= (own[i] > -INFINITY && in(own[i], id(i / 4, i % 4)) ? 1u : 0u) << i;
+            done(bits, 0);
         } else
             for (int j0 = 0; j0 < steps; j0 += 8) {
                 float v[32];
 #pragma unroll
                 for (int j = 0; j < 8; j++) load(j0 + j, v, 4 * j);
+                uint32_t bits = 0;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { const float w = v[4 * j + e]; f(w > -INFINITY ? w : -INFINITY, id(j0 + j, e)); }
+                for (int i = 0; i < 32; i++) bits |= (v[i] > -INFINITY && in(v[i], id(j0 + i / 4, i % 4)) ? 1u : 0u) << i;
+                done(bits, j0);
             }
-    }
-    // a bit for each of the thread's values (in registers) that reaches `least`
-    __device__ __forceinline__ uint32_t reach(float least) const {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < VPT; i++) bits |= (own[i] >= least && own[i] > -INFINITY ? 1u : 0u) << i;
-        return bits;
     }
     // f(value, id) of the thread's values that are there
     template <class F> __device__ __forceinline__ void each(F && f) const {
@@ -508,7 +501,7 @@ template <int VPT, bool WIDE> struct sp_values {
     }
 };
 // The ranks of the values with a bit into `list`, in any order, while there is room; `count` goes up by how many there are.  A few of a row: what is listed is read once more, and the code is short (with a ballot and the store for each of
-// a thread's 32 values, all of it code that runs once, the list of 40 of 32000 took 8000 clocks)
+// a thread's 32 values, all of it code that runs once, the list of 40 of 32000 took 8000 clocks and takes 4800)
 template <class F> static __device__ __forceinline__ void sp_list_few(uint32_t bits, int * count, int room, sp_u64 * list, const float * x, F && id_of) {
     const int lane = threadIdx.x & 63, n = __popc(bits), upto = (int) pi_wave_scan((uint32_t) n), all = __builtin_amdgcn_readlane(upto, 63);
     if (all == 0) return;
@@ -526,14 +519,7 @@ template <class S, class F> static __device__ __forceinline__ int sp_gather(cons
     __syncthreads();
     if (threadIdx.x == 0) L.n = 0;
     __syncthreads();
-    X.every([&](float v, int id) __attribute__((always_inline)) {
-        const unsigned long long who = __ballot(v > -INFINITY && in(v, id));
-        if (who == 0) return;                                // (the wave together)
-        int at = 0;
-        if ((threadIdx.x & 63) == (unsigned) __builtin_ctzll(who)) at = atomicAdd(&L.n, __popcll(who));
-        at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + sp_rank_in(who);
-        if ((who >> (threadIdx.x & 63) & 1) && at < SP_LIST) L.list[at] = sp_rank(v, id);
-    });
+    X.marked(in, [&](uint32_t bits, int j0) __attribute__((always_inline)) { sp_list_few(bits, &L.n, SP_LIST, L.list, X.x, [&](int i) __attribute__((always_inline)) { return X.id(j0 + i / 4, i % 4); }); });
     __syncthreads();
     return L.n;
 }
@@ -620,7 +606,6 @@ template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sa
     sp_row R(A, row, L.table);
     const sp_values<VPT, WIDE> X(R.x, R.V);
     sp_table(L.table);
-    if (tid == 0) L.n = 0;
     if (pi_aborted_together(gone, abort_w)) return;
     // the largest value, a thread's and everybody's, and a bound that at least k of them reach
     float mine = -INFINITY; int mine_id = 0;
@@ -629,9 +614,7 @@ template <int VPT, bool WIDE> __global__ void __launch_bounds__(SP_THREADS) k_sa
     sp_u64 top = 0;
     if (few) {                                               // (the largest comes with the list)
         const float least = sp_at_least(sp_wave_bound<SP_WAVES>(bounds, mine, R.k));
-        sp_list_few(X.reach(least), &L.n, SP_LIST, L.list, R.x, [&](int i) __attribute__((always_inline)) { return X.id(i / 4, i % 4); });
-        __syncthreads();
-        const int n = L.n;
+        const int n = sp_gather(X, L, [&](float v, int) __attribute__((always_inline)) { return v >= least; });
         if (n == 0) {
             if (tid == 0) sp_leave(A, row, -1, 0.0f, 0);
             return;
