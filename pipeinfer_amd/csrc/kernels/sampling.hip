@@ -846,15 +846,10 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
     __syncthreads();
     sp_slice * mine = S.slices + (int64_t) row * slices + slice;
     sp_u64 * list = S.lists + ((int64_t) row * slices + slice) * SP_SLICE_LIST;
+    uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const unsigned long long who = __ballot(x[e] > rest.listed && !(x[e] > rest.above));
-        if (who == 0) continue;
-        int at = 0;
-        if (lane == __builtin_ctzll(who)) at = atomicAdd(&listed, __popcll(who));
-        at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + sp_rank_in(who);
-        if ((who >> lane & 1) && at < SP_SLICE_LIST) list[at] = sp_rank(x[e], sp_slice_id<WIDE>(base, e / 4, e % 4));
-    }
+    for (int e = 0; e < 16; e++) bits |= (x[e] > rest.listed && !(x[e] > rest.above) ? 1u : 0u) << e;
+    sp_list_few(bits, &listed, SP_SLICE_LIST, list, R.x, [&](int e) __attribute__((always_inline)) { return sp_slice_id<WIDE>(base, e / 4, e % 4); });
     if (R.k == 0) {                                          // (top-k: the list is all that is asked for)
         const bool once = R.cooled == 1.0, few_stay = R.min_p > 0.0f;
         const double top = (double) R.top;
