@@ -130,7 +130,7 @@ struct px_args {
     int row_blocks, prompt_parts, own_blocks, own_parts;     // of a key head's rows; parts that the prompt is cut into; blocks of 32 of a token's rows; parts of the cells behind it
     px_div by_group, by_kv, by_row_blocks, by_own_blocks, by_own_parts, by_parts, by_quads;
     int prompt_share, own_share;                             // cells, words of the mask of a part where the sizes are the arguments'
-    bool together;                                           // the prompt's workgroups take the own cells too
+    bool wide, together;                                     // blocks of 128 rows; the prompt's workgroups take the own cells too
     float * parts_o; float2 * parts_ml;                      // [part][token][head][dim], [part][token][head] (maximum, sum)
     float * out; int64_t out_stride; float * lse;
 };
@@ -460,14 +460,16 @@ __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts
 }
 
 // ---- how the work is cut ---------------------------------------------------------------------------------------------------------------------------------------------------------------
-static bool px_wide_rows(int rows) { return rows > 64; }
 // device: the sizes are the device's, which may leave cells behind the prompt where the arguments leave none
 static void px_plan(px_args & A, bool device) {
     const int rows = A.n_tok * A.group, target = 2 * pi_cu_count();
-    const bool wide = px_wide_rows(rows);
-    A.row_blocks = wide ? (rows + 127) / 128 : (rows + 31) / 32;
     A.own_blocks = (A.group + 31) / 32;
-    const int64_t units = (int64_t) A.kv * A.row_blocks, own = (int64_t) A.n_tok * A.kv * A.own_blocks;
+    const int64_t own = (int64_t) A.n_tok * A.kv * A.own_blocks, narrow = (int64_t) A.kv * ((rows + 31) / 32);
+    // More than 64 rows go by 128, four waves past the same tiles, where there is work for it - scores times values from 2^31 on (64 tokens of 64 / 8 heads of 128 values: 8000 cells 46 us, by 32 rows 56; 4000 cells 34 and 34; 2000 cells
+    // 30 and 25) - or where blocks of 32 rows and the tokens' own cells would be more workgroups than run at once (100 tokens of 32 heads with keys of their own, 600 cells: 21 us and 24; 200 of 64 / 8 heads, 1000 cells: 28 and 34)
+    A.wide = rows > 64 && (narrow + own / 4 > target || (double) A.kv * rows * A.prompt * A.dim > 0x1p31);
+    A.row_blocks = A.wide ? (rows + 127) / 128 : (rows + 31) / 32;
+    const int64_t units = (int64_t) A.kv * A.row_blocks;
     const int words = (A.n_kv + 31) / 32 - A.prompt / 32;
     // Of the prompt two workgroups a compute unit where each has 1024 cells and more (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 129 us, with one 139), else one, since every part is written and read once more (32 such tokens,
     // 8000 cells: 33 us, with two 41; 1 token, 16000 cells: 23 and 25), and 256 cells and more in each (24 tokens of 32 heads, 2047 cells: 18 us, with 128 cells 23).  Of a token's own cells four waves' worth of what is left of two
@@ -519,7 +521,7 @@ template <int DP> static int px_launch(const px_args & A, hipStream_t s) {
     const int parts = A.prompt_parts + A.own_parts, nta = std::min(A.n_tok, PI_KT_MAXNT - 1), acct = pi_account_n_kv() > 0 ? pi_account_n_kv() : A.n_kv;
     const double bytes = 4.0 * acct * A.row + 6.0 * A.n_tok * A.heads * A.dim;
     if (blocks > 0) {
-        if (px_wide_rows(A.n_tok * A.group)) PI_KT_LAUNCH(PI_KT_ATT, 0, nta, bytes, (k_prefix_attention<DP, true>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
+        if (A.wide) PI_KT_LAUNCH(PI_KT_ATT, 0, nta, bytes, (k_prefix_attention<DP, true>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
         else PI_KT_LAUNCH(PI_KT_ATT, 0, nta, bytes, (k_prefix_attention<DP, false>), dim3((unsigned) blocks), dim3(256), 0, s, A, pi_abort_word());
         PI_CHECK_LAUNCH();
     }

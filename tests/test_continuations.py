@@ -174,6 +174,36 @@ def test_attention(heads, kv, dim, tokens, prompt, own):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(32, 32, 24, 70, 333, 90), (32, 32, 64, 70, 129, 40), (32, 32, 80, 70, 31, 300), (32, 32, 128, 70, 100, 70), (32, 32, 160, 70, 65, 33), (32, 32, 256, 67, 90, 63), (32, 32, 40, 70, 1, 257),
+                                                             (32, 32, 64, 70, 0, 50), (32, 32, 96, 129, 97, 0), (16, 16, 128, 128, 300, 20)])
+def test_attention_of_many_rows(heads, kv, dim, tokens, prompt, own):
+    """as many workgroups as go by 128 rows; the same with sizes that the device knows, and scores far apart"""
+    U, lib = gpu()
+    rng = np.random.default_rng(dim)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own)
+    want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
+    for room in (None, (prompt + 500, prompt + own + 900)):
+        if room:
+            k, v = (np.concatenate([x, np.full((room[1] - len(x), kv, dim), np.nan, np.float16)]) for x in (k, v))
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5, room)
+        p.attend()
+        got, lse = p.outputs()
+        check_attention(got, want, lse, want_lse)
+    q[...] = 1.0
+    for slope in (0.5, 40.0):
+        k[:prompt] = (np.arange(prompt)[:, None, None] * (slope / dim)).astype(np.float16)
+        p = Pass(U, lib, q, k, v, seen, prompt, 1.0, room)
+        p.attend()
+        got, lse = p.outputs()
+        want, want_lse, _ = soft_max(q, k, v, seen, 1.0)
+        # (scores of up to 2^14: the factor log2(e) and the difference are rounded at 2^-24 of them, the sum of dim <= 256 equal products of 11 bits is exact)
+        far = 2 ** -24 * 3 * max(1.0, np.abs(want_lse[np.isfinite(want_lse)]).max())
+        assert np.linalg.norm(got - want) <= max(FAR, far) * np.linalg.norm(want) and (np.isneginf(lse) == np.isneginf(want_lse)).all()
+        some = np.isfinite(want_lse)
+        assert np.abs(lse[some] - want_lse[some]).max(initial=0.0) <= max(LSE_FAR, far)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("prompt,own", [(0, 1 << 20), (1 << 20, 0), (600000, 500000)])
 def test_a_million_cells_of_one_head(prompt, own):
     """as many parts of a row as there can be; the values are positive, so that an output's error is the weights'"""
