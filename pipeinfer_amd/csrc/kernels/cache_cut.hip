@@ -344,7 +344,7 @@ template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base
 }
 
 // An array's address stands in the kernel's arguments, in host memory: that read is most of a short move, 3 us for one workgroup's, and the reads of all of them queue (45 arrays of 1000 rows, 331 moving: 1440 workgroups of 256 threads 18 us,
-// 45 of 1024 9).  So a workgroup takes 1024 rows of one array
+// 45 of 1024 9).  So a workgroup takes 1024 rows of one array.  Long moves are bound by memory (32 arrays, half of 32768 rows of 2 KB kept: 229 us, 1.07 GB at 4.7 TB/s)
 __global__ void __launch_bounds__(1024) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int blocks, int keep, int cells, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w)) return;
     __shared__ int2 lists[16][64];

@@ -327,6 +327,9 @@ static __device__ __forceinline__ void px_share(int n, int share, int part, int 
 // a share of n things in whole runs of `run`, so that `parts` of them are all
 static __host__ __device__ __forceinline__ int px_share_of(int n, int run, int parts) { const uint32_t runs = ((uint32_t) n + run - 1) / run; return (int) ((runs + parts - 1) / parts) * run; }
 
+// Many rows and cells are bound by the matrix cores and the vector unit in turns (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 120 us, 101 GFLOP with the weights' second halves, 840 TFLOP/s; of the clocks 45 % matrix, 40 % vector:
+// the registers of two waves are full, so little of one runs under the other); keys of their own for every head by the caches' rows (24 tokens, 2047 cells, 51 MB: 15 us, 3.4 TB/s); what lies between by the chain of a workgroup's few tiles
+// (16 tokens of 64 / 8 heads, 4000 cells, 22 MB: 15 us - 3 until the first rows are there, 5 for four runs of 32 cells a wave, 2 to meet; a token of 32 / 4 heads of 64 values, 513 cells: 8 us)
 template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;                      // (what a wave takes from LDS as an index, it has put there itself)
     constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 4 * 32 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
@@ -398,9 +401,9 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
     else px_leave<DP>(A, S, part, tok, head, in < rows, g);
 }
 
-#define PX_PARTS 1088                                            /* what k_prefix_merge has room for; the prompt takes two of a compute unit's at most */
+#define PX_PARTS 1088       /* what k_prefix_merge has room for; the prompt takes two of a compute unit's at most */
 // The parts' sums over their joint maximum.  Four of a row's values to a thread and about every `groups`-th part, the threads of a row meet in LDS: with a wave per row and its parts one after the other the loads' latency was all the
-// time (4096 rows of 17 parts: 24.2 us; 1024 of 17: 20.8)
+// time (4096 rows of 17 parts: 24.2 us; 1024 of 17: 20.8).  Bound by the parts' rows (4096 rows of 17: 12.0 us, 38 MB at 3.2 TB/s; 768 of 9: 4.0)
 __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts, int log_groups, int rows_here, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;
     __shared__ float2 ml[PX_PARTS];                         // (512 of them at most where the workgroup has more than one row)
@@ -565,6 +568,8 @@ extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, co
 
 // ---- what cells are given ---------------------------------------------------------------------------------------------------------------------------------------------------------------
 // A wave keeps the keys of 64 cells as operands and the queries of the rows go past it, 64 at a time through LDS for the four waves: a lane has 32 cells of one row of 32, adds their weights up row after row, and the lanes meet at the end.
+// Bound by the clocks of the matrix cores (27 %) and the vector unit (49 %: a factor, an exponential and a sum for every score), which hardly run at once: 64 tokens of 64 / 8 heads of 128 values, 16000 cells 46 us, 17 GFLOP.  With the cells
+// on the lanes, one sum for each and a third fewer instructions, and with three waves of it on a SIMD, the time was the same, under masks 8 % longer.  8 tokens of 32 heads, 3000 cells: 10 us, the chain from the arguments to the first keys
 struct pm_args {
     const uint16_t * q; int64_t q_stride;
     const uint16_t * k; int64_t row;
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, 
 static void pm_plan(pm_args & A) {
     const int rows = A.n_tok * A.group;
     A.cell_blocks = (A.n_kv + 255) / 256;
-    // as many parts of the rows as leave the fewest workgroup rounds of the chip's two per compute unit idle, at most one for every 64 rows
+    // as many parts of the rows as leave the fewest workgroup rounds of the chip's two per compute unit idle, at most one for every 64 rows (64 tokens of 64 / 8 heads, 16000 cells: two parts 48 us, four 58, eight 78)
     const int64_t units = (int64_t) A.cell_blocks * A.kv, slots = 2 * pi_cu_count();
     A.row_parts = 1;
     double least = 1e30;
