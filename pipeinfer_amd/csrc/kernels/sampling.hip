@@ -8,7 +8,7 @@
 //
 // Sums are whole numbers, weights in steps of 2^-44 (a row of 2^19 of the largest weight fits 64 bits): the order of additions, and with it of atomics, is without effect, and a sum is off by less than the number of its terms x 2^-45
 // of a total of at least 1.  Exponentials are fp64, within 1e-13: with fp32's the borders of thousands of candidates would move by whole tokens.
-// Rows of up to 32768 logits: a workgroup each, the values in registers (k_sample).  Bound by the steps one after the other, code that runs once for the most part (1 row of 32000, top-k 40: 12 us; 64 of 32768, top-p 0.95: 39).
+// Rows of up to 32768 logits: a workgroup each, the values in registers (k_sample).  Bound by the steps one after the other, code that runs once for the most part (1 row of 32000, top-k 40: 11 us; 64 of 32768, top-p 0.95: 39).
 //   few of the best (top_k up to 128): what every wave has its sixteenth of top_k lanes above bounds the top_k-th from below; what reaches the bound - a few times top_k values - is listed in LDS, ranked there, and one wave does the rest
 //   any number: the weights are added up in bins of equal width below the maximum, the bin that holds the border is listed and ranked
 // Longer rows in slices of 8192, so that a few of them fill the chip, in four launches (4 rows of 32768 by a workgroup each: top-k 20 10.9 us, top-p 0.95 36; of 50000 in slices 15.3 and 32):
@@ -654,7 +654,7 @@ template <bool WIDE, int STEPS> static __device__ __forceinline__ void sp_slice_
     }
 }
 
-// Bound by the logits (256 rows of 131072: 30 us, 4.4 TB/s; 64 rows 16 us, the bins' atomics behind the only round of loads; 33 rows of 65024, lists alone, 9)
+// Bound by the logits (256 rows of 131072: 30 us, 4.4 TB/s; 64 rows 16 us, the bins' atomics behind the only round of loads; 33 rows of 65024, lists alone, 6.5)
 template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
     __shared__ uint32_t bins[SP_COARSE], bounds[8];
@@ -730,7 +730,7 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     if (slice == 0 && tid == 0) S.rest[row].zero = R.zero;
 }
 
-// Bound by its steps one after the other (64 rows of 131072 8 us, 33 rows of 65024 with their lists 10)
+// Bound by its steps one after the other (64 rows of 131072 8 us, 33 rows of 65024 with their lists 11)
 __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x;
     __shared__ sp_shared L;
