@@ -34,8 +34,8 @@
 #define SP_RUN 512           /* values whose chances are added up by themselves */
 #define SP_RUNS (SP_SLICE / SP_RUN)
 #define SP_COARSE 2048       /* a slice's bins */
-#define SP_COARSE_UNIT 64.0f
-#define SP_AHEAD 8.0f        /* how far above the largest of the row's first 1024 values they begin: 24 units are left below it */
+#define SP_COARSE_UNIT 64.0f /* of them to a unit of logits, or twice to sixteen times as many (sp_unit) */
+#define SP_AHEAD 512.0f      /* how many lie above the largest of the row's first 1024 values: 24 units below it are left at 64 to a unit */
 #define SP_POOL 8192         /* entries of a row's lists of few */
 #define SP_SLICE_LIST 512
 #define SP_REGISTERS 32768   /* longest row whose values stay in a workgroup's registers */
@@ -110,7 +110,7 @@ struct sp_args {
 
 // what the launches over slices hand on: values above `above` are added up, those above `listed` listed; joined 0: left to one workgroup
 struct sp_slice { sp_u64 best, listed, weights, above, kept, chances[SP_RUNS]; double over; };
-struct sp_rest { sp_u64 best; float zero, above, listed; int32_t open, joined, pad; };
+struct sp_rest { sp_u64 best; float zero, above, listed; int32_t open, joined; float unit; };
 static int sp_slices(int vocab) { return (vocab + SP_SLICE - 1) / SP_SLICE; }
 struct sp_scratch { sp_rest * rest; sp_slice * slices; sp_u64 * lists; uint32_t * bins; };          // [row], [row][slice], [row][slice][SP_SLICE_LIST], [row][slice][SP_COARSE]
 
@@ -146,13 +146,13 @@ static __device__ __forceinline__ sp_u64 sp_before(sp_u64 v, sp_shared & L, int 
 // a row's settings, and what is known of it so far
 struct sp_row {
     const float * x; int V; float top_p, min_p; double cooled; bool greedy; int k; const double * table;
-    float top, zero; sp_u64 best, last;                      // the first of the order; where the bins begin; nothing below the rank `last` stays
+    float top, zero, unit; sp_u64 best, last;                // the first of the order; where the bins begin; the slices' bins to a unit; nothing below the rank `last` stays
     __device__ __forceinline__ sp_row(const sp_args & A, int row, const double * t) : table(t) {
         x = A.logits + (int64_t) row * A.stride; V = A.vocab;
         const float temp = A.temp ? A.temp[row] : 1.0f;
         top_p = A.top_p ? A.top_p[row] : 1.0f; min_p = A.min_p ? A.min_p[row] : 0.0f; k = A.top_k ? A.top_k[row] : 0;
         greedy = !(temp > 0.0f); cooled = greedy ? 1.0 : 1.0 / (double) temp;
-        top = zero = 0.0f; best = last = 0;
+        top = zero = 0.0f; unit = SP_COARSE_UNIT; best = last = 0;
         if (k < 0 || k >= V) k = 0;
         if (min_p > 1.0f) k = 1;                             // (nothing reaches it: the first alone)
     }
@@ -165,7 +165,7 @@ struct sp_row {
     __device__ __forceinline__ int bin(float v) const { return (int) fminf(v >= zero ? 0.0f : (zero - v) * SP_PER_UNIT, (float) (SP_BINS - 1)); }
     // the slices' bins, from `zero` on, a value's place in its bin in `rest`; what is no number or not there: the last
     __device__ __forceinline__ int coarse(float v, float & rest) const {
-        const float d = __builtin_amdgcn_fmed3f((zero - v) * SP_COARSE_UNIT, 0.0f, (float) SP_COARSE - 0.5f), f = floorf(d);
+        const float d = __builtin_amdgcn_fmed3f((zero - v) * unit, 0.0f, (float) SP_COARSE - 0.5f), f = floorf(d);
         rest = d - f;
         return (int) f;
     }
@@ -177,6 +177,9 @@ struct sp_row {
     __device__ __forceinline__ sp_u64 share(float v, int id) const { return greedy ? (sp_rank(v, id) == best ? sp_steps(1.0) : 0) : sp_steps(chance(v)); }
     __device__ __forceinline__ float part(float v, sp_u64 sum) const { return (float) ((greedy ? 1.0 : chance(v)) * SP_ONE / (double) sum); }
 };
+// Bins to a unit where the first 1024 values lie `spread` apart: the bins below the largest of them reach one and a half times that.  (64 rows of 250000 of deviation 1, top-p 0.95: of 64 bins to a unit one holds 1600, the lists are full and
+// the rows go to a workgroup each, 754 us; of 128 to a unit 76)
+static __device__ __forceinline__ float sp_unit(float spread) { return SP_COARSE_UNIT * (spread <= 1.0f ? 16.0f : spread <= 2.0f ? 8.0f : spread <= 4.0f ? 4.0f : spread <= 8.0f ? 2.0f : 1.0f); }
 // the step of the sum that u falls on
 static __device__ __forceinline__ sp_u64 sp_drawn(float u, sp_u64 sum) {
     const double want = (double) u * (double) sum;
@@ -659,7 +662,7 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
     __shared__ uint32_t bins[SP_COARSE], bounds[8];
     __shared__ sp_u64 tops[4];
-    __shared__ float firsts[4];
+    __shared__ float firsts[4], lows[4];
     __shared__ double overs[4];
     __shared__ int listed;
     __shared__ double table[SP_TABLE];
@@ -667,12 +670,12 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     sp_row R(A, row, table);
     // (the row's last values for the last slice, so that its waves are as full as the others': the fewer lanes, the lower a bound.  What stands in the slice before is taken out once the bound is known)
     const int begin = slice * SP_SLICE, from = min(begin, R.V - SP_SLICE), base = from + wave * (SP_SLICE / 4);
-    float x[32], first = -INFINITY;
+    float x[32], first = -INFINITY, low = INFINITY;
     sp_slice_load<WIDE, 8>(R, base, x);
     const bool few = R.k > 0 && R.k <= 128, border = !few && (R.k > 0 || R.nucleus());
     if (border)
 #pragma unroll
-        for (int e = 0; e < 4; e++) first = fmaxf(first, R.x[256 * e + tid]);          // (rows are longer)
+        for (int e = 0; e < 4; e++) { const float v = R.x[256 * e + tid]; first = fmaxf(first, v); low = fminf(low, v > -INFINITY ? v : INFINITY); }         // (rows are longer)
     if (tid == 0) listed = 0;
     if (pi_aborted_together(gone, abort_w)) return;
     sp_slice * mine_of = S.slices + (int64_t) row * slices + slice;
@@ -698,8 +701,8 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     }
     own_ones();
     sp_u64 top = sp_wave_top(mine > -INFINITY ? sp_rank(mine, mine_id) : 0);
-    first = pi_wave_max(first);
-    if (lane == 0) { tops[wave] = top; firsts[wave] = first; }
+    first = pi_wave_max(first); low = -pi_wave_max(-low);
+    if (lane == 0) { tops[wave] = top; firsts[wave] = first; lows[wave] = low; }
     if (border) sp_table(table);
     if (border)
 #pragma unroll
@@ -708,16 +711,19 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     if (tid == 0) mine_of->best = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
     if (!border) return;
     first = fmaxf(fmaxf(firsts[0], firsts[1]), fmaxf(firsts[2], firsts[3]));
-    R.zero = (first > -INFINITY && first < INFINITY ? first : 0.0f) + SP_AHEAD;
+    low = fminf(fminf(lows[0], lows[1]), fminf(lows[2], lows[3]));
+    R.unit = sp_unit(first - low);
+    R.zero = (first > -INFINITY && first < INFINITY ? first : 0.0f) + SP_AHEAD / R.unit;
     const bool counts = R.k > 0;
+    const float step = 1.0f / R.unit;
     double over = 0.0;                                       // the weights of what lies above the bins
 #pragma unroll
     for (int e = 0; e < 32; e++) {
         if (!counts && __any(x[e] > R.zero)) { if (x[e] > R.zero) { over += sp_exp((double) x[e] - (double) R.zero, table); continue; } }
         float rest;
         const int b = R.coarse(x[e], rest);
-        const float r = rest * (1.0f / SP_COARSE_UNIT);
-        // (of e^-r 16 bits, r < 1/64: 8192 of them fit a bin; the series up to r^3 / 6, the next term: 2^-29)
+        const float r = rest * step;
+        // (of e^-r 16 bits, r <= 1/64: 8192 of them fit a bin; the series up to r^3 / 6, the next term: 2^-29)
         const uint32_t w = counts ? 1u : (uint32_t) fmaf(65536.0f, 1.0f - r * fmaf(-r, fmaf(r, -1.0f / 6.0f, 0.5f), 1.0f), 0.5f);
         if (x[e] > -INFINITY) atomicAdd(&bins[b], w);
     }
@@ -727,7 +733,7 @@ template <bool WIDE> __global__ void __launch_bounds__(256) k_sample_slice(const
     uint32_t * to = S.bins + ((int64_t) row * slices + slice) * SP_COARSE;
 #pragma unroll
     for (int i = 0; i < SP_COARSE / 1024; i++) *(uint4 *) (to + 1024 * i + 4 * tid) = *(const uint4 *) (bins + 1024 * i + 4 * tid);
-    if (slice == 0 && tid == 0) S.rest[row].zero = R.zero;
+    if (slice == 0 && tid == 0) { S.rest[row].zero = R.zero; S.rest[row].unit = R.unit; }
 }
 
 // Bound by its steps one after the other (64 rows of 131072 8 us, 33 rows of 65024 with their lists 11)
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
         if (tid == 0) *rest = sp_rest{ best, R.top, -INFINITY, -INFINITY, 1, R.top < INFINITY, 0 };
         return;
     }
-    const float zero = rest->zero;
+    const float zero = rest->zero, unit = rest->unit;
     // two bins to a thread, over the slices
     const uint32_t * from = S.bins + (int64_t) row * slices * SP_COARSE + 2 * tid;
     sp_u64 a = 0, b = 0;
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
         __syncthreads();
         lo = 0; hi = R.k <= SP_BEST ? L.hit : -1;
     } else {
-        const float each = 1.44269504f / SP_COARSE_UNIT, far = fmaxf((R.top - zero) * 1.44269504f, 0.0f);            // (relative to what is largest)
+        const float each = 1.44269504f / unit, far = fmaxf((R.top - zero) * 1.44269504f, 0.0f);            // (relative to what is largest)
         double over = 0.0;
         if (tid == 0 && far > 0.0f) for (int i = 0; i < slices; i++) over += of[i].over;
         const double wa = (double) a * (double) __builtin_amdgcn_exp2f(-each * (float) (2 * tid) - far) + over * 65536.0 * (double) __builtin_amdgcn_exp2f(-far);
@@ -825,9 +831,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
         lo = (int) L.answer; hi = (int) L.before;
     }
     // (far below an infinity, or bins that end too high: no)
-    const bool joined = R.top - zero <= 100.0f && hi >= 0 && hi < SP_COARSE - 1 && fabsf(zero) < 32768.0f;
+    const bool joined = R.top - zero <= 100.0f && hi >= 0 && hi < SP_COARSE - 1 && fabsf(zero) * unit < 32768.0f * SP_COARSE_UNIT;
     // (half a bin further down: every value of bin hi is listed, whichever way its difference was rounded)
-    if (tid == 0) *rest = sp_rest{ best, zero, lo == 0 ? INFINITY : zero - (float) lo / SP_COARSE_UNIT, zero - ((float) hi + 1.5f) / SP_COARSE_UNIT, 1, joined, 0 };
+    if (tid == 0) *rest = sp_rest{ best, zero, lo == 0 ? INFINITY : zero - (float) lo / unit, zero - ((float) hi + 1.5f) / unit, 1, joined, unit };
 }
 
 // Sums of a run in fp64, in an order that is always the same, then in steps.  Bound by its instructions, the fp64 ones for the most part: 22 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, so 22 us;

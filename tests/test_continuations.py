@@ -383,7 +383,7 @@ def test_rows_that_move(cells, keep, sizes):
         assert np.array_equal(d.get(np.uint8, a.shape), want)
 
 
-def sampled(x, temp, top_k, top_p, min_p, u):
+def sampled(x, temp, top_k, top_p, min_p, u, clear=1e-9):
     x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
     order = np.argsort(-x, kind="stable")
     order = order[x[order] > -np.inf]
@@ -403,7 +403,7 @@ def sampled(x, temp, top_k, top_p, min_p, u):
         edge = np.float64(top_p) * w.sum()
         n = max(1, int((ahead < edge).sum()))
         near = np.abs(ahead / edge - 1).min() if edge > 0 else 1.0
-        sure &= bool(near > 1e-9 or top_p <= 0)
+        sure &= bool(near > clear or top_p <= 0)
         order, w = order[:n], w[:n]
     n = max(1, int((w >= np.float64(min_p)).sum())) if min_p > 0 else len(order)
     order = order[:n]
@@ -429,11 +429,11 @@ def run_sample(U, lib, x, vocab, settings, u):
     return [o.get(t) for o, t in zip(out, (np.int32, np.float32, np.int32))]
 
 
-def check_sample(U, lib, x, vocab, settings, u):
+def check_sample(U, lib, x, vocab, settings, u, clear=1e-9):
     got = run_sample(U, lib, x, vocab, settings, u)
     full = [np.full(len(x), v) if s is None else np.asarray(s) for s, v in zip(settings, (1.0, 0, 1.0, 0.0))]
     for t in range(len(x)):
-        i, p, n, sure = sampled(x[t, :vocab], np.float32(full[0][t]), int(full[1][t]), np.float32(full[2][t]), np.float32(full[3][t]), np.float32(u[t]))
+        i, p, n, sure = sampled(x[t, :vocab], np.float32(full[0][t]), int(full[1][t]), np.float32(full[2][t]), np.float32(full[3][t]), np.float32(u[t]), clear)
         assert sure, ("an input at a border", t)                         # (no test asks which side of a border a sum falls that two roundings could move)
         assert got[0][t] == i and got[2][t] == n and abs(got[1][t] - p) <= 2.0 ** -23 * p, (t, [f[t] for f in full], u[t], got[0][t], i, got[2][t], n, got[1][t], p)
 
@@ -456,6 +456,29 @@ def test_sample(vocab, stride):
         check_sample(U, lib, x, vocab, (np.full(rows, 1.3), None, np.full(rows, 0.9), None), u)
         check_sample(U, lib, x, vocab, (None, None, None, np.full(rows, 0.05)), u)
         check_sample(U, lib, x, vocab, (rng.choice([0.0, 0.5, 1.0, 2.0, -1.0], rows), rng.choice([0, 1, 2, 50, 128, 129, 1000, 200000, -3], rows), rng.choice([0.0, 0.3, 0.8, 0.99, 1.0, 2.0], rows), rng.choice([0.0, 0.02, 0.3, 1.0], rows)), u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread", [0.01, 0.1, 0.5, 1.0, 2.0])
+def test_sample_of_flat_rows(spread):
+    """logits that lie close together, a few far above them, in front or behind, or two crowds; the border among them"""
+    U, lib = gpu()
+    rng = np.random.default_rng(int(spread * 100))
+    V = 100001
+    x = (spread * rng.standard_normal((8, V))).astype(np.float32)
+    x[1, 90000] += 30 * spread
+    x[2, 5] += 20 * spread
+    x[3, 50000:50100] += 9 * spread
+    x[4, ::2] -= 12 * spread
+    x[5, 2000:] -= 30 * spread
+    x[6] += 1000.0
+    x[7, rng.random(V) < 0.9] = -np.inf
+    x[7, :1100] = -np.inf
+    # (Weights here are off by 1.4e-13 of themselves, the first term that their series leaves out, and a few 2^-53; a sum by that and by 2^-45 for each of its 200 runs, relative to a total of 1 and more: 6e-12 at most.  numpy's own sums of
+    # 100001 terms: 17 halvings x 2^-53 and, one after the other, 10^5 x 2^-53 = 1.1e-11 in cumsum at the very worst, its square root's part as a rule.  The weights at the border of 0.9999 are 1e-8 of the total: 2e-11 keeps clear of both)
+    for p in (0.3, 0.95, 0.9999):
+        check_sample(U, lib, x, V, (np.full(8, 0.9), None, np.full(8, p), None), rng.random(8), 2e-11)
+    check_sample(U, lib, x, V, (None, np.full(8, 700), np.full(8, 0.9), None), rng.random(8))
 
 
 @pytest.mark.gpu
