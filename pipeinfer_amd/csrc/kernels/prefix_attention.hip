@@ -600,8 +600,17 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) key[u][i] = px_chunk(k, 16 * i + 8 * g, A.dim);
     }
+    const bool masked = cells0 + 256 > prompt, own = A.mask && n_kv > prompt;             // (without a mask nobody sees a cell behind the prompt)
     float next_lse = INFINITY;
+    uint32_t ahead[2][2] = {};                                 // the mask's words of the rows on their way, lane n's row, the wave's two blocks of cells
     auto load = [&](int r) __attribute__((always_inline)) {
+        if (masked && own)
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const uint32_t * row = A.mask + (int64_t) px_quotient((uint32_t) min(r + 32 * v + n, r1 - 1), A.by_group) * words;
+#pragma unroll
+                for (int u = 0; u < 2; u++) ahead[v][u] = row[min(mine / 32 + u, words - 1)];
+            }
 #pragma unroll
         for (int i = 0; i < N; i++) {
             // (past the head's end the keys are zero; what is multiplied there is the head's first values)
@@ -621,12 +630,12 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         if (tid < 64) lse[to][tid] = next_lse;
     };
     px_f32x16 sum[2] = { px_zero(), px_zero() };
-    const bool masked = cells0 + 256 > prompt, own = A.mask && n_kv > prompt;             // (without a mask nobody sees a cell behind the prompt)
     if (r0 < r1) { load(r0); store(0); }
     int cur = 0;
     for (int r = r0; r < r1; r += 64, cur ^= 1) {
         __syncthreads();
         const bool more = r + 64 < r1;
+        const uint32_t sees[2][2] = { { ahead[0][0], ahead[0][1] }, { ahead[1][0], ahead[1][1] } };
         if (more) load(r + 64);
         // (cells that every row sees have no test: half of the vector instructions are exponentials' then)
         auto rows = [&](auto with_mask) __attribute__((always_inline)) {
@@ -642,7 +651,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
                     if constexpr (with_mask) {
                         bits = 0;
                         if (base < n_kv) {
-                            if (own && base + 32 > prompt) bits = A.mask[(int64_t) px_quotient((uint32_t) min(r + 32 * v + n, r1 - 1), A.by_group) * words + base / 32];
+                            if (own && base + 32 > prompt) bits = sees[v][u];
                             if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
                             if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
                         }
