@@ -344,15 +344,16 @@ template <class T> static __device__ __forceinline__ void cm_rows(uint8_t * base
 }
 
 // An array's address stands in the kernel's arguments, in host memory: that read is most of a short move, 3 us for one workgroup's, and the reads of all of them queue (45 arrays of 1000 rows, 331 moving: 1440 workgroups of 256 threads 18 us,
-// 45 of 1024 9).  So a workgroup takes 1024 rows of one array.  Long moves are bound by memory (32 arrays, half of 32768 rows of 2 KB kept: 229 us, 1.07 GB at 4.7 TB/s)
-__global__ void __launch_bounds__(1024) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int blocks, int keep, int cells, const int32_t * __restrict__ abort_w) {
+// 45 of 1024 9).  So a workgroup takes 1024 rows of one array, or fewer, down to 64, while they
+// hold more than a megabyte and there are fewer than two workgroups a compute unit (80 arrays of 1000 rows of 8 KB, half of them moving: 164 us, of 1024 rows 248; 4 of 2500 such rows 25 and 95).  Long moves are bound by memory (32 arrays, half of 32768 rows of 2 KB kept: 229 us, 1.07 GB at 4.7 TB/s)
+__global__ void __launch_bounds__(1024) k_cache_move(const cm_arrays A, const int32_t * __restrict__ source, int blocks, int of_wave, int keep, int cells, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w)) return;
     __shared__ int2 lists[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, array = (int) blockIdx.x / blocks, block = (int) blockIdx.x % blocks;
     uint8_t * base = A.at[array];
     const uint64_t bytes = A.bytes[array];
-    const int64_t row64 = ((int64_t) block * 16 + wave) * 64 + lane;
-    const int row = (int) min(row64, (int64_t) keep), from = row < keep ? source[row] : -1;
+    const int64_t row64 = ((int64_t) block * 16 + wave) * of_wave + lane;
+    const int row = (int) min(row64, (int64_t) keep), from = lane < of_wave && row < keep ? source[row] : -1;
     const bool moves = from >= keep && from < cells;
     const unsigned long long who = __ballot(moves);
     if (moves) lists[wave][__popcll(who & ((1ull << lane) - 1))] = make_int2(row, from);
@@ -372,10 +373,13 @@ extern "C" int pi_op_cache_move(void * const * arrays, const int64_t * row_bytes
         cm_arrays A{};
         const int n = std::min(CM_ARRAYS, n_arrays - i0);
         double bytes = 0;
-        for (int i = 0; i < n; i++) { A.at[i] = (uint8_t *) arrays[i0 + i]; A.bytes[i] = (uint64_t) row_bytes[i0 + i]; bytes += 2.0 * std::min(keep, cells - keep) * row_bytes[i0 + i]; }
-        const int blocks = (keep + 1023) / 1024;
+        int64_t largest = 0;
+        for (int i = 0; i < n; i++) { A.at[i] = (uint8_t *) arrays[i0 + i]; A.bytes[i] = (uint64_t) row_bytes[i0 + i]; largest = std::max(largest, row_bytes[i0 + i]); bytes += 2.0 * std::min(keep, cells - keep) * row_bytes[i0 + i]; }
+        int of_wave = 64;                                    // rows
+        while (of_wave > 4 && (int64_t) n * ((keep + 16 * of_wave - 1) / (16 * of_wave)) < 2 * pi_cu_count() && largest * 16 * of_wave > 1 << 20) of_wave /= 2;
+        const int blocks = (keep + 16 * of_wave - 1) / (16 * of_wave);
         if ((int64_t) n * blocks > 0x7fffffff) { pi_set_error("pi_op_cache_move: %d rows of %d arrays", keep, n); return -1; }
-        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) (n * blocks)), dim3(1024), 0, (hipStream_t) stream, A, source, blocks, keep, cells, pi_abort_word());
+        PI_KT_LAUNCH(PI_KT_OTHER, 0, 1, bytes, k_cache_move, dim3((unsigned) (n * blocks)), dim3(1024), 0, (hipStream_t) stream, A, source, blocks, of_wave, keep, cells, pi_abort_word());
         PI_CHECK_LAUNCH();
     }
     return 0;

@@ -363,7 +363,7 @@ def test_choice(cells):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("cells,keep,sizes", [(1000, 700, [4, 512, 2064, 6, 1, 16384, 12]), (300, 20, [2048] * 130 + [4]), (5000, 2500, [160, 80, 4])])
+@pytest.mark.parametrize("cells,keep,sizes", [(1000, 700, [4, 512, 2064, 6, 1, 16384, 12]), (300, 20, [2048] * 130 + [4]), (5000, 2500, [160, 80, 4]), (400, 250, [65536, 16384, 70000, 2]), (3001, 1500, [8192, 512])])
 def test_rows_that_move(cells, keep, sizes):
     """rows of every alignment, more arrays than a launch takes; entries that point in front of the budget or behind the cache move nothing"""
     U, lib = gpu()
