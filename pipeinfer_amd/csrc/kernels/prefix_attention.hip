@@ -378,7 +378,7 @@ template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 
         whose = px_quotient(c, A.by_own_parts);
         if (whose >= (uint32_t) A.n_tok) return;
         kvh = (int) (unit - a * A.kv); tok = (int) whose; part = (int) (c - whose * A.own_parts); in = (int) (a - c * A.own_blocks) * 32 + n; head = kvh * A.group + min(in, A.group - 1);
-        px_share(w_all, A.dyn ? px_share_of(w_all, 8, A.own_parts) : A.own_share, part, from, to);
+        px_share(w_all, A.dyn ? px_share_of(w_all, 2, A.own_parts) : A.own_share, part, from, to);
         part += A.prompt_parts;
         px_queries<DP>(A, q, tok, head, g);
         px_start(S);
@@ -476,7 +476,8 @@ static void px_plan(px_args & A, bool device) {
     const int words = (A.n_kv + 31) / 32 - A.prompt / 32;
     // Of the prompt two workgroups a compute unit where each has 1024 cells and more (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 129 us, with one 139), else one, since every part is written and read once more (32 such tokens,
     // 8000 cells: 33 us, with two 41; 1 token, 16000 cells: 23 and 25), and 256 cells and more in each (24 tokens of 32 heads, 2047 cells: 18 us, with 128 cells 23).  Of a token's own cells four waves' worth of what is left of two
-    // workgroups a compute unit, 16 words of the mask and more each
+    // workgroups a compute unit; of the mask 16 words and more each, fewer for few tokens, whose words are fuller (64 / 8 heads of 128 values: 1 token of 400 cells 12 us by 2 words, 20 by 16; 4 tokens of 400 10.6 by 4, 11.2 by 8, 13.0 by 16;
+    // 8 of 200 behind 1000 17 by 2, 13.0 by 8 and 13.2 by 16)
     A.prompt_parts = A.own_parts = 0;
     A.prompt_share = A.own_share = 1;
     if (A.prompt > 0) {
@@ -491,7 +492,8 @@ static void px_plan(px_args & A, bool device) {
     else if (A.n_kv > A.prompt) {
         const int64_t left = std::max<int64_t>(4 * (target - A.prompt_parts * units), own);          // (waves of workgroups that run beside the prompt's)
         const int64_t most = std::min<int64_t>(left / own, PX_PARTS - A.prompt_parts);
-        A.own_share = px_share_of(words, 8, (int) std::max<int64_t>(1, std::min<int64_t>(most, (words + 15) / 16)));
+        const int least = std::min(16, 2 * A.n_tok);
+        A.own_share = px_share_of(words, 2, (int) std::max<int64_t>(1, std::min<int64_t>(most, (words + least - 1) / least)));
         A.own_parts = (words + A.own_share - 1) / A.own_share;
     } else if (device && A.prompt > 0) A.own_parts = 1;
     A.by_group = px_divide_by(A.group); A.by_kv = px_divide_by(A.kv); A.by_row_blocks = px_divide_by(std::max(1, A.row_blocks)); A.by_own_blocks = px_divide_by(A.own_blocks); A.by_own_parts = px_divide_by(std::max(1, A.own_parts));
