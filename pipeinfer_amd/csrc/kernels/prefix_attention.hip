@@ -570,7 +570,7 @@ extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, co
 
 // ---- what cells are given ---------------------------------------------------------------------------------------------------------------------------------------------------------------
 // A wave keeps the keys of 64 cells as operands and the queries of the rows go past it, 64 at a time through LDS for the four waves: a lane has 32 cells of one row of 32, adds their weights up row after row, and the lanes meet at the end.
-// Bound by the clocks of the matrix cores (27 %) and the vector unit (49 %: a factor, an exponential and a sum for every score), which hardly run at once: 64 tokens of 64 / 8 heads of 128 values, 16000 cells 46 us, 17 GFLOP.  With the cells
+// Bound by the clocks of the matrix cores (27 %) and the vector unit (49 %: a factor, an exponential and a sum for every score), which hardly run at once: 64 tokens of 64 / 8 heads of 128 values, 16000 cells 43 us, 17 GFLOP.  With the cells
 // on the lanes, one sum for each and a third fewer instructions, and with three waves of it on a SIMD, the time was the same, under masks 8 % longer.  8 tokens of 32 heads, 3000 cells: 10 us, the chain from the arguments to the first keys
 struct pm_args {
     const uint16_t * q; int64_t q_stride;
@@ -707,7 +707,8 @@ __global__ void __launch_bounds__(256) k_mass_merge(const pm_args A, int parts, 
 static void pm_plan(pm_args & A) {
     const int rows = A.n_tok * A.group;
     A.cell_blocks = (A.n_kv + 255) / 256;
-    // as many parts of the rows as leave the fewest workgroup rounds of the chip's two per compute unit idle, at most one for every 64 rows (64 tokens of 64 / 8 heads, 16000 cells: two parts 48 us, four 58, eight 78)
+    // as many parts of the rows as leave the fewest workgroup rounds of the chip's two per compute unit idle, at most one for every 64 rows (64 tokens of 64 / 8 heads of 128 values, 1000 cells: one part 24 us, four 11, eight 12; 4000 cells 24, 15 and 18; 16000
+    // cells one or two parts 46 .. 50 us, eight 75)
     const int64_t units = (int64_t) A.cell_blocks * A.kv, slots = 2 * pi_cu_count();
     A.row_parts = 1;
     double least = 1e30;
