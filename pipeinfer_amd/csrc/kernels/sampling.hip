@@ -40,6 +40,7 @@
 #define SP_SLICE_LIST 512
 #define SP_REGISTERS 32768   /* longest row whose values stay in a workgroup's registers */
 #define SP_ONE 17592186044416.0    /* 2^44 */
+#define SP_HALF 0x1p-45      /* half a step: a weight up to here is none (sp_steps) */
 #define SP_MAX_VOCAB (1 << 19)
 
 typedef unsigned long long sp_u64;
@@ -209,7 +210,7 @@ template <class F> static __device__ __forceinline__ int sp_reach(sp_shared & L,
     return L.hit;
 }
 
-// the token in the values [from, to), of which `t` of the sum is left.  (A run's sum may be a few steps above its values': then it is the last of them)
+// the token in the values [from, to), of which `t` of the sum is left.  (A run's sum may be above its values', which are rounded one by one: then it is the last of them.  What is no step by itself is not in the sum either, so one of them has a share)
 static __device__ __forceinline__ void sp_pick(const sp_args & A, const sp_row & R, int row, int from, int to, sp_u64 t, sp_u64 sum, int kept) {
     const int lane = threadIdx.x & 63;
     int last = -1;
@@ -836,7 +837,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
     if (tid == 0) *rest = sp_rest{ best, zero, lo == 0 ? INFINITY : zero - (float) lo / unit, zero - ((float) hi + 1.5f) / unit, 1, joined, unit };
 }
 
-// Sums of a run in fp64, in an order that is always the same, then in steps.  Bound by its instructions, the fp64 ones for the most part: 22 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, so 22 us;
+// Sums of a run in fp64, in an order that is always the same, then in steps; of the chances without those that are no step by themselves, so that no run of nothing but such ones is drawn.  Bound by its instructions, the fp64 ones for the most part: 22 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, so 22 us;
 // exponentials by two and three workgroups on a compute unit 21.5, four with spilled registers 28)
 template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
@@ -885,7 +886,7 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
                     sp_exp4(d, w, table);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) chance += stays[e] ? w[e] : 0.0;
+                for (int e = 0; e < 4; e++) chance += stays[e] && w[e] > SP_HALF ? w[e] : 0.0;
             }
             const sp_u64 c = sp_sum_steps(pi_wave_sum_f64(chance));
             if (lane == 0) mine->chances[2 * wave + run] = c;

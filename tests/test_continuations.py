@@ -666,3 +666,29 @@ def test_captured_and_beside_each_other():
             assert all(np.array_equal(a, b) for a, b in zip(results(p), want)), i
         step(passes[i % 2], None)
         L.check(lib.pi_device_sync(), "sync")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [32768, 40000, 40001, 131072])
+def test_sample_where_runs_of_ids_are_too_unlikely_to_be_drawn(vocab):
+    """hundreds of neighbours whose chances round to nothing one by one but not together: none of them is drawn, and every output is written, whatever u falls on"""
+    U, lib = gpu()
+    rng = np.random.default_rng(vocab)
+    x = np.zeros((8, vocab), np.float32)
+    x[0, -1] = 32.0                                                      # 0.22 of a step each, 114 steps in 512 of them
+    x[1, -1] = 31.3
+    x[2, vocab // 2] = 36.0
+    x[3] = 0.3 * rng.standard_normal(vocab); x[3, -3] = 34.0
+    x[4, :vocab // 2] = -34.0; x[4, vocab // 2:] = rng.standard_normal(vocab - vocab // 2)
+    x[5, -1] = 3.2                                                       # (at a temperature of 0.1 as far)
+    x[6, 600] = 3.3; x[6, 700:] = -np.inf
+    x[7] = -33.0; x[7, rng.integers(0, vocab, 40)] = rng.standard_normal(40)
+    temp = np.array([1, 1, 1, 1, 1, 0.1, 0.1, 1], np.float32)
+    for u in (0.0, 2.0 ** -40, 2.0 ** -24, 0.5, 1 - 2.0 ** -24):
+        got = run_sample(U, lib, x, vocab, (temp, None, None, None), [u] * 8)
+        for t in range(8):
+            i, p, n, sure = sampled(x[t], temp[t], 0, np.float32(1.0), np.float32(0.0), np.float32(u))
+            assert sure or u == 2.0 ** -40, (u, t)                       # (2^-40: sixteen whole steps, where sums of whole steps leave no doubt)
+            assert got[0][t] == i and got[2][t] == n and abs(got[1][t] - p) <= 2.0 ** -23 * p, (t, u, got[0][t], i, got[2][t], n, got[1][t], p)
+    # behind a nucleus: of the crowd 3.2 below the largest about a quarter stays
+    check_sample(U, lib, x[5:6], vocab, (temp[5:6], None, np.full(1, 0.25), None), [0.0])
