@@ -869,10 +869,10 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
         for (int run = 0; run < 2; run++) {
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                double d[4], w[4];
+                double below[4], d[4], w[4];
                 bool stays[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) { const float v = run ? x[8 + 4 * half + e] : x[4 * half + e]; d[e] = fmax((double) v - top, -600.0); stays[e] = v > rest.above; }
+                for (int e = 0; e < 4; e++) { const float v = run ? x[8 + 4 * half + e] : x[4 * half + e]; below[e] = (double) v - top; d[e] = fmax(below[e], -600.0); stays[e] = v > rest.above; }
                 sp_exp4(d, w, table);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -882,7 +882,7 @@ template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const
                 }
                 if (!once && !R.greedy) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) d[e] = fmax(d[e] * R.cooled, -600.0);
+                    for (int e = 0; e < 4; e++) d[e] = fmax(below[e] * R.cooled, -600.0);          // (of what is far below the largest a high temperature leaves something)
                     sp_exp4(d, w, table);
                 }
 #pragma unroll

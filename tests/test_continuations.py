@@ -692,3 +692,18 @@ def test_sample_where_runs_of_ids_are_too_unlikely_to_be_drawn(vocab):
             assert got[0][t] == i and got[2][t] == n and abs(got[1][t] - p) <= 2.0 ** -23 * p, (t, u, got[0][t], i, got[2][t], n, got[1][t], p)
     # behind a nucleus: of the crowd 3.2 below the largest about a quarter stays
     check_sample(U, lib, x[5:6], vocab, (temp[5:6], None, np.full(1, 0.25), None), [0.0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1000, 32768, 40000, 131075])
+def test_sample_at_high_temperatures(vocab):
+    """logits hundreds and thousands below the largest, at temperatures at which they are drawn"""
+    U, lib = gpu()
+    rng = np.random.default_rng(vocab + 1)
+    x = -3000.0 * rng.random((6, vocab)).astype(np.float32)
+    x[1, ::2] = -np.inf
+    x[2, vocab // 2:] -= 1e5
+    temp = np.array([800.0, 300.0, 5e4, 1e6, 150.0, 2000.0], np.float32)
+    for _ in range(3):
+        check_sample(U, lib, x, vocab, (temp, None, None, None), rng.random(6))
+    check_sample(U, lib, x, vocab, (temp, None, None, np.full(6, 0.001)), rng.random(6))
