@@ -6,7 +6,8 @@
 // The query rows of a key head - tokens x its query heads - are one matrix against the prompt's keys, so a key is read once for all of them.  The cells behind the prompt differ from token to token: a workgroup takes one
 // token's, listed from its mask, and reads no other, so that what stands in the others is without effect.  Scores are computed transposed (rows = cells): what a lane then holds - sixteen cells of one query - is, eight at a time, the
 // operand of the product with the values, and the values come from LDS through its transposing load.
-// Sums and statistics are fp32.  Products are fp16 x fp16 (exact in fp32); a weight is two fp16 values, what the first leaves and the second again cuts off (22 bits; one alone, 11 bits, is 1.4e-4 off over 32000 cells).
+// Sums and statistics are fp32.  Products are fp16 x fp16 (exact in fp32); a weight is two fp16 values, rounded to nearest, the second one what the first leaves (23 bits; one alone, 11 bits, is 1.4e-4 off over 32000 cells).  fp16 ends at
+// 2^-24, so weights are held relative to a power of two that follows them: up when they no longer fit, and down again behind a cell that took nearly all (px_weigh)
 #include "ops_common.h"
 #include "kernel_timing.h"
 #include "wave_scan.h"
@@ -16,7 +17,8 @@
 #include <type_traits>
 
 typedef _Float16 px_half8 __attribute__((ext_vector_type(8)));
-typedef __fp16 px_half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 px_half2 __attribute__((ext_vector_type(2)));
+typedef float px_f32x2 __attribute__((ext_vector_type(2)));
 typedef short px_short4 __attribute__((ext_vector_type(4)));
 typedef uint32_t px_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t px_u32x2 __attribute__((ext_vector_type(2)));
@@ -31,16 +33,27 @@ static __device__ __forceinline__ int px_cell(int i, int g) { return 8 * (i >> 2
 // Bytes between rows in LDS.  Keys: an odd number of 16 bytes, so that the rows of a read of 16 bytes a lane lie apart.  Values: a transposing read takes 64 bytes of four rows for 32 lanes: 64 or 192 modulo 256
 template <int DP> struct px_lds { static constexpr int K = 2 * DP + 16, V = (DP / 32) % 2 ? 2 * DP : 2 * DP + 64; };
 
-#define PX_LIFT 6.0f        /* weights are held times 2^6 or more: fp16's smallest steps are then 2^-30 of the largest weight */
-#define PX_MOST 32768.0f    /* the maximum that weights are relative to follows when those of a lane's sixteen cells exceed this: fp16 holds them until then */
+// What weights are relative to, in powers of two.  (Tiles that are weighed twice: of scores of a deviation of up to two, and one cell far above them, one or two of a walk; of a deviation of four 8 of 32 and 10 of 100: 64 tokens of 64 / 8
+// heads of 128 values, 32000 cells 126 us instead of 122, 100 tokens of 64 heads of 64 values, 4000 cells 37 instead of 32)
+#define PX_MOST 65504.0f    /* a lane's weights of sixteen cells: fp16 holds them up to here, then it rises, */
+#define PX_FULL 4096.0f     /* ... where weights are looked at, from here on: */
+#define PX_TOP 4.0f         /* so that the tile's largest is 2^4, which leaves room for the next tiles', */
+#define PX_ALONE 14.0f      /* or 2^14, where hardly another of the tile's is within */
+#define PX_GAP 20.0f        /*    2^20 of it */
+#define PX_LEAST 0.125f     /* it may fall when they are this or less */
+#define PX_FALL 7.0f        /* ... and the largest less than 2^-7, and rounded, at 2^-25, at 2^-18 of itself: so that it is 2^4 */
+#define PX_HELD 60.0f       /* ... while the sums stay below 2^60: what is smaller beside them is lost to fp32 anyway */
+#define PX_ROSE 4           /* rises of a walk that are looked behind */
 #define PX_LIST 2048        /* cells of 64 words of a mask, a wave's */
 
-// 32 queries of one key head, a column of the tile per lane, lanes l and l + 32 the same: their sums so far.  Of acc the outputs 32 j + px_cell(i, g); m in powers of two, l of the lane's own cells
+// 32 queries of one key head, a column of the tile per lane, lanes l and l + 32 the same: their sums so far.  Of acc the outputs 32 j + px_cell(i, g); weights are 2^(score - m), l the sum of those of the lane's own cells (0: none)
 template <int DP> struct px_sums { px_f32x16 acc[DP / 32]; float m, l; };
+// of a walk over tiles: the next one, the one at which weights are looked at, rises that may still be looked behind
+struct px_looks { int tile = 0, look = 0, spare = PX_ROSE; };
 template <int DP> static __device__ __forceinline__ void px_start(px_sums<DP> & S) {
 #pragma unroll
     for (int j = 0; j < DP / 32; j++) S.acc[j] = px_zero();
-    S.m = -INFINITY; S.l = 0.0f;
+    S.m = S.l = 0.0f;
 }
 
 // scores of which the first `live` cells of the tile count
@@ -53,34 +66,44 @@ static __device__ __forceinline__ void px_only(px_f32x16 & s, int live, int g) {
 struct px_weights { px_u32x4 hi[2], lo[2]; };
 static __device__ __forceinline__ void px_no_weights(px_weights & P) { for (int z = 0; z < 2; z++) P.hi[z] = P.lo[z] = px_u32x4{ 0, 0, 0, 0 }; }
 
-// of a tile's scores the weights and their sum; c = scale * log2(e).  S holds the products of the tiles before
-template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & S, px_weights & P, const px_f32x16 & s, float c) {
-    float p[16], l, minus = -1.0f;
+// Of a tile's scores the weights and their sum; c = scale * log2(e).  S holds the products of the tiles before.
+// What weights are relative to is not the largest score: any power of two is as good that keeps them within fp16, the sums are fp32.  It rises when a lane's weights no longer fit.  A cell far above the others would leave those only fp16's
+// last bits, and where its values are small they are what the outputs are made of: so it falls again where a tile's weights are small.  That is looked for at tiles 0, 1, 5, 21, .. and behind the first rises, not at every tile: scores that
+// are far apart from tile to tile would have it follow them up and down.  (One cell of 20 above 32000 others, its values zero: 7e-7 off; relative to the largest score, both halves cut off, 1.4e-3)
+template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & S, px_looks & W, px_weights & P, const px_f32x16 & s, float c) {
+    float p[16], l = 0.0f, minus = -1.0f;
     asm("" : "+v"(minus));                                   // (unknown to the compiler: a - h would be a conversion and a subtraction, fma takes the fp16 as it is)
     auto weigh = [&]() __attribute__((always_inline)) {
-        const float lift = PX_LIFT - (S.m == -INFINITY ? 0.0f : S.m);
 #pragma unroll
-        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, lift));
+        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -S.m));
         l = (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) + (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
 #pragma unroll
         for (int z = 0; z < 2; z++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float a = p[8 * z + 2 * e], b = p[8 * z + 2 * e + 1];
-                const px_half2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
+                const px_half2 h = __builtin_convertvector((px_f32x2{ a, b }), px_half2);
                 P.hi[z][e] = __builtin_bit_cast(uint32_t, h);
-                P.lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float) h[0], minus, a), fmaf((float) h[1], minus, b)));
+                P.lo[z][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((px_f32x2{ fmaf((float) h[0], minus, a), fmaf((float) h[1], minus, b) }), px_half2));
             }
     };
     weigh();
-    // (the maximum is looked for where a lane's weights say that it has grown, or that there was none: it costs a dozen instructions a tile)
-    if (__any(l > PX_MOST || S.m == -INFINITY)) {
-        float top = s[0];
+    const bool looks = W.tile == W.look;
+    const float most = looks ? PX_FULL : PX_MOST, least = looks ? PX_LEAST : 0.0f;
+    if (looks) W.look = 4 * W.tile + 1;
+    if (__any(l > most || l <= least)) {
+        float top = fmaxf(s[0], s[1]), next = fminf(s[0], s[1]);          // (next: one cell far above the others is not in it)
 #pragma unroll
-        for (int i = 1; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
-        top = fmaxf(top, s[15]);
+        for (int i = 2; i < 16; i += 2) { top = fmaxf(fmaxf(top, s[i]), s[i + 1]); next = fmaxf(next, fminf(s[i], s[i + 1])); }
         top = fmaxf(top, pi_partner<32>(top)) * c;
-        const float m = fmaxf(S.m, top), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);
+        next = fmaxf(next, pi_partner<32>(next)) * c;
+        const float both = fmaxf(l, pi_partner<32>(l)), sum = S.l + pi_partner<32>(S.l);
+        float m = S.m;
+        const bool rises = both > most;
+        if (rises) m = top - (top - next > PX_GAP ? PX_ALONE : PX_TOP);
+        else if (both <= least && top < m - PX_FALL && top > -INFINITY) m = fmaxf(top - PX_TOP, m - PX_HELD + __builtin_amdgcn_logf(sum));
+        if (W.spare > 0 && !looks && __any(rises)) { W.look = W.tile + 1; W.spare--; }
+        const float f = sum == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);
         S.m = m; S.l *= f;
 #pragma unroll
         for (int j = 0; j < DP / 32; j++)
@@ -89,6 +112,7 @@ template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & 
         weigh();
     }
     S.l += l;
+    W.tile++;
 }
 
 // the values' operand from rows of `stride` bytes in LDS: at = the wave's first row + px_value_at; sixteen lanes take four rows of sixteen values and each gets a column
@@ -146,7 +170,7 @@ template <int DP> static __device__ __forceinline__ void px_leave(const px_args 
     if (last) {
         o = A.out + (int64_t) tok * A.out_stride + (int64_t) head * A.dim;
         f = l == 0.0f ? 0.0f : 1.0f / l;
-        if (g == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (S.m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+        if (g == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (S.m + __builtin_amdgcn_logf(l)) * 0.693147181f;
     } else {
         const int64_t at = (int64_t) part * A.n_tok * A.heads + r;
         o = A.parts_o + at * A.dim;
@@ -228,6 +252,7 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
     __syncthreads();
     px_f32x16 s = scores(0);
     px_weights P;
+    px_looks W;
     px_no_weights(P);
     const int value_at = 32 * KS + px_value_at(lane, VS);
     for (int t = 0; t < tiles; t++) {
@@ -238,7 +263,7 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
         // (of the first tile no weights: its own values times 0; behind the last one the scores of whatever stands there, for nobody)
         px_products<DP, VS>(S, P, lds + (max(t - 1, 0) & 3) * TILE + value_at);
         const px_f32x16 next = scores(t + 1);
-        px_weigh<DP>(S, P, s, A.c);
+        px_weigh<DP>(S, W, P, s, A.c);
         s = next;
     }
     px_products<DP, VS>(S, P, lds + (tiles - 1 & 3) * TILE + value_at);
@@ -263,6 +288,7 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
         }
     };
     if (first >= count) return;
+    px_looks W;
     load(first);
     for (int at = first; at < count; at += step) {
         px_u32x4 kc[N];
@@ -280,7 +306,7 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
         for (int i = 0; i < N; i++) s = px_mfma(kc[i], q[i], s);
         if (at + 32 > count) px_only(s, count - at, g);
         px_weights P;
-        px_weigh<DP>(S, P, s, A.c);
+        px_weigh<DP>(S, W, P, s, A.c);
         px_products<DP, VS>(S, P, vt);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -310,7 +336,7 @@ template <int DP> static __device__ __forceinline__ void px_meet(const px_args &
     const int64_t r = (int64_t) tok * A.heads + head, to = (int64_t) part * A.n_tok * A.heads + r;
     if (wave == 0 && g == 0 && mine) {
         if (!last) A.parts_ml[to] = make_float2(m, l);
-        else if (A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+        else if (A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147181f;
     }
     if (!mine || (l == 0.0f && !last)) return;               // (k_prefix_merge leaves such a part out)
     float * o = last ? A.out + (int64_t) tok * A.out_stride + (int64_t) head * A.dim : A.parts_o + to * A.dim;
@@ -330,11 +356,11 @@ static __host__ __device__ __forceinline__ int px_share_of(int n, int run, int p
 // Many rows and cells are bound by the matrix cores and the vector unit in turns (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 120 us, 101 GFLOP with the weights' second halves, 840 TFLOP/s; of the clocks 45 % matrix, 40 % vector:
 // the registers of two waves are full, so little of one runs under the other); keys of their own for every head by the caches' rows (24 tokens, 2047 cells, 51 MB: 15 us, 3.4 TB/s); what lies between by the chain of a workgroup's few tiles
 // (16 tokens of 64 / 8 heads, 4000 cells, 22 MB: 15 us - 3 until the first rows are there, 5 for four runs of 32 cells a wave, 2 to meet; a token of 32 / 4 heads of 64 values, 513 cells: 8 us)
-template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
+template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;                      // (what a wave takes from LDS as an index, it has put there itself)
     constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 4 * 32 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
     __shared__ __attribute__((aligned(16))) uint8_t lds[NARROW > WIDE_B ? NARROW : WIDE_B];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, g = lane >> 5;
     const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv);
     const uint32_t pairs = (uint32_t) A.kv * A.prompt_parts, prompt_blocks = pairs * A.row_blocks;
     px_u32x4 q[DP / 16];
@@ -459,7 +485,7 @@ __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t r = r0 + mine;
     *(px_f32x4 *) (A.out + r / A.heads * A.out_stride + r % A.heads * A.dim + d) = o * f;
-    if (d == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m - PX_LIFT + __builtin_amdgcn_logf(l)) * 0.693147181f;
+    if (d == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147181f;
 }
 
 // ---- how the work is cut ---------------------------------------------------------------------------------------------------------------------------------------------------------------

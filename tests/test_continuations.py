@@ -707,3 +707,34 @@ def test_sample_at_high_temperatures(vocab):
     for _ in range(3):
         check_sample(U, lib, x, vocab, (temp, None, None, None), rng.random(6))
     check_sample(U, lib, x, vocab, (temp, None, None, np.full(6, 0.001)), rng.random(6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens", [(4, 4, 64, 4), (8, 1, 128, 2), (8, 2, 80, 70), (300, 300, 8, 65)])
+@pytest.mark.parametrize("prompt,above,spread", [(1500, 11.9, 0.0), (8000, 11.2, 0.0), (8000, 11.2, 0.5), (8000, 16.0, 2.0), (32000, 15.0, 0.0), (32000, 16.0, 1.0), (32000, 20.0, 2.0)])
+def test_a_cell_that_takes_nearly_all(heads, kv, dim, tokens, prompt, above, spread):
+    """one cell far above the others with nothing in its values, in front, behind or between: what the others give is as exact as without it"""
+    if heads == 300 and prompt > 8000:
+        prompt, above = 4000, above - 2.0
+    U, lib = gpu()
+    rng = np.random.default_rng(prompt + heads + int(above))
+    for at in (0, prompt // 3, prompt - 1):
+        q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, 0)
+        q[:, :, 1:] = spread * rng.standard_normal(q[:, :, 1:].shape)
+        q[:, :, 0] = 4.0
+        k, v = k[:prompt], (0.5 + rng.random((prompt, kv, dim))).astype(np.float16)
+        k[:, :, 0] = 0.0
+        k[at] = 0.0
+        k[at, :, 0] = above / 4 * dim ** 0.5
+        v[at] = 0.0
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5)
+        p.attend()
+        got, lse = p.outputs()
+        want, want_lse = np.zeros(got.shape), np.zeros(lse.shape)
+        for j in range(heads):
+            s = q[:, j].astype(np.float64) @ k[:, j * kv // heads].astype(np.float64).T * dim ** -0.5
+            want_lse[:, j] = m = np.log(np.exp(s - s.max(1, keepdims=True)).sum(1)) + s.max(1)
+            want[:, j] = np.exp(s - m[:, None]) @ v[:, j * kv // heads].astype(np.float64)
+        # (Beside FAR and LSE_FAR: where the others are all equal, a sum that the one cell has made large is rounded the same way at every one of its up to prompt / 32 additions, by up to 2^-24 of it.  Else those go either way)
+        same = 0.0 if spread else 2.0 ** -24 * ((prompt + 31) // 32)
+        assert np.isfinite(got).all() and np.linalg.norm(got - want) <= (FAR + same) * np.linalg.norm(want) and np.abs(lse - want_lse).max() <= LSE_FAR + same
