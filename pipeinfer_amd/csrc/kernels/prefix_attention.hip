@@ -214,7 +214,8 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
     px_sums<DP> S;
     px_start(S);
     const uint16_t * k = A.k + kvh * A.dim, * v = A.v + kvh * A.dim;
-    // (a chunk past the head's end reads its first: the queries are zero there, and such outputs do not leave)
+    // (a chunk past the head's end reads its first, and is not stored: zeros stand there, as in the queries - an infinity of the keys would make no number of them)
+    auto in_head = [&](int i) __attribute__((always_inline)) { return min(i * 256 + tid, 32 * CH - 1) % CH * 8 < A.dim; };
     auto load = [&](int t) __attribute__((always_inline)) {
         const int64_t c = c0 + 32 * t;
         const uint16_t * kc = k + c * A.row, * vc = v + c * A.row;
@@ -232,10 +233,19 @@ template <int DP> static __device__ __forceinline__ void px_wide(const px_args &
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int x = min(i * 256 + tid, 32 * CH - 1);
+            if (!in_head(i)) continue;
             *(px_u32x4 *) (to + x / CH * KS + x % CH * 16) = kr[i];
             *(px_u32x4 *) (to + 32 * KS + x / CH * VS + x % CH * 16) = vr[i];
         }
     };
+    if (A.dim < DP)
+#pragma unroll 1
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int x = min(i * 256 + tid, 32 * CH - 1);
+                if (!in_head(i)) *(px_u32x4 *) (lds + t * TILE + x / CH * KS + x % CH * 16) = *(px_u32x4 *) (lds + t * TILE + 32 * KS + x / CH * VS + x % CH * 16) = px_u32x4{ 0, 0, 0, 0 };
+            }
     auto scores = [&](int t) __attribute__((always_inline)) {
         const uint8_t * kt = lds + (t & 3) * TILE + n * KS + 16 * g;
         px_f32x16 s = px_zero();
@@ -298,6 +308,9 @@ template <int DP, class C> static __device__ __forceinline__ void px_walk(const 
             const int x = i * 64 + lane;
             *(px_u32x4 *) (mine + x / CH * VS + x % CH * 16) = vr[i];
         }
+        if (A.dim < DP)                                      // (as the queries there: an infinity of the keys' first values would make no number of them; the least that goes by DP is DP - 56)
+#pragma unroll
+            for (int i = N > 4 ? N - 4 : 0; i < N; i++) if (16 * i + 8 * g >= A.dim) kc[i] = px_u32x4{ 0, 0, 0, 0 };
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         if (at + step < count) load(at + step);
         const uint8_t * vt = mine + px_value_at(lane, VS);

@@ -738,3 +738,26 @@ def test_a_cell_that_takes_nearly_all(heads, kv, dim, tokens, prompt, above, spr
         # (Beside FAR and LSE_FAR: where the others are all equal, a sum that the one cell has made large is rounded the same way at every one of its up to prompt / 32 additions, by up to 2^-24 of it.  Else those go either way)
         same = 0.0 if spread else 2.0 ** -24 * ((prompt + 31) // 32)
         assert np.isfinite(got).all() and np.linalg.norm(got - want) <= (FAR + same) * np.linalg.norm(want) and np.abs(lse - want_lse).max() <= LSE_FAR + same
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(32, 4, 64, 1, 200, 13), (4, 4, 72, 24, 100, 70), (8, 1, 40, 16, 129, 40), (71, 1, 24, 1, 0, 700), (24, 3, 200, 9, 1, 257), (16, 2, 80, 8, 1000, 0), (2, 1, 256, 3, 40, 0),
+                                                             (32, 32, 80, 70, 333, 0), (32, 32, 40, 70, 333, 20), (300, 300, 8, 65, 333, 0), (16, 16, 160, 128, 300, 20)])
+def test_keys_of_minus_infinity(heads, kv, dim, tokens, prompt, own):
+    """a seen key whose score is minus infinity takes its cell out, and nothing else changes, in heads of every length"""
+    U, lib = gpu()
+    rng = np.random.default_rng(dim + heads)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own, loners=tokens > 1)
+    q[:, :, 0] = q[:, :, 1] = 0.5 + rng.random((tokens, heads))
+    for i, c in enumerate(rng.permutation(np.flatnonzero(seen.any(0)))[:4]):
+        k[c, :, i % 2] = -np.inf
+    want, want_lse, w = soft_max(q, k, v, seen, dim ** -0.5)
+    assert np.isfinite(want).all() and np.isfinite(want_lse).any()
+    p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5)
+    p.attend()
+    got, lse = p.outputs()
+    check_attention(got, want, lse, want_lse)
+    p.lse = U.Dev(want_lse.astype(np.float32))
+    mass = U.Dev(np.zeros(prompt + own, np.float32))
+    p.give(mass, 0.0)
+    assert np.allclose(mass.get(np.float32), w.sum((0, 1))[:prompt + own], rtol=8e-6, atol=1e-12)
