@@ -159,6 +159,39 @@ struct px_args {
     float * out; int64_t out_stride; float * lse;
 };
 
+// Outputs that are no finite numbers although the sum of the weights `l` is: a value that the token sees is infinite, and one of a weight's two halves was zero.  They are the sum of what is not finite among its values.
+// o: the token's outputs of the head; from `d` on, every step-th four.  (Off the way: a thread reads the values of all cells, eight at a time)
+static __device__ __forceinline__ bool px_finite(float x) { return fabsf(x) < INFINITY; }
+static __device__ __forceinline__ bool px_finite(px_f32x4 x) { return px_finite(x[0]) && px_finite(x[1]) && px_finite(x[2]) && px_finite(x[3]); }
+static __device__ __forceinline__ void px_infinite(const px_args & A, float * o, int tok, int head, int d, int step) {
+    const int n_kv = A.dyn ? max(0, min(A.dyn[1], A.n_kv)) : A.n_kv, prompt = min(A.dyn ? max(0, min(A.dyn[0], A.prompt)) : A.prompt, n_kv), n = A.mask ? n_kv : prompt;
+    const uint32_t * mask = A.mask + (int64_t) tok * ((A.n_kv + 31) / 32);
+    for (; d < A.dim; d += step) {
+        px_f32x4 x = *(px_f32x4 *) (o + d), sum = { 0.0f, 0.0f, 0.0f, 0.0f };
+        if (px_finite(x)) continue;
+        const uint16_t * v = A.v + head / A.group * A.dim + d;
+#pragma unroll 1
+        for (int c0 = 0; c0 < n; c0 += 8) {
+            px_u32x2 of[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) of[i] = *(const px_u32x2 *) (v + (int64_t) min(c0 + i, n - 1) * A.row);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int c = min(c0 + i, n - 1);
+                const bool sees = c < prompt || (mask[c >> 5] >> (c & 31) & 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = (float) __builtin_bit_cast(_Float16, (uint16_t) (of[i][e >> 1] >> (16 * (e & 1))));
+                    if (sees && !px_finite(y)) sum[e] += y;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) if (!px_finite(x[e]) && sum[e] != 0.0f) x[e] = sum[e];
+        *(px_f32x4 *) (o + d) = x;
+    }
+}
+
 // the sums of 32 rows of key head j from row0 on: part `part` of theirs, or the result where it is the only one
 template <int DP> static __device__ __forceinline__ void px_leave(const px_args & A, px_sums<DP> & S, int part, int tok, int head, bool mine, int g) {
     const float l = S.l + pi_partner<32>(S.l);
@@ -187,6 +220,13 @@ template <int DP> static __device__ __forceinline__ void px_leave(const px_args 
             }
     };
     if (A.dim == DP) leave(std::true_type{}); else leave(std::false_type{});
+    if (!last || !(l > 0.0f) || !px_finite(l)) return;
+    float all = 0.0f;                                        // (no number, or 0)
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) all = fmaf(S.acc[j][i], 0.0f, all);
+    if (all != 0.0f) px_infinite(A, o, tok, head, 4 * g, 8);
 }
 
 // values d .. d + 7 of a row of `dim`, zeros behind its end (read without a branch: behind one, a load is waited for where the branches meet)
@@ -353,12 +393,17 @@ template <int DP> static __device__ __forceinline__ void px_meet(const px_args &
     }
     if (!mine || (l == 0.0f && !last)) return;               // (k_prefix_merge leaves such a part out)
     float * o = last ? A.out + (int64_t) tok * A.out_stride + (int64_t) head * A.dim : A.parts_o + to * A.dim;
+    bool odd = false;
 #pragma unroll
     for (int k = 0; k < DP / 32; k++) {
         const int i = 4 * k + wave, d = 8 * i + 4 * g;
         const px_f32x4 a = at[(i * 4) * 64 + lane], b = at[(i * 4 + 1) * 64 + lane], c = at[(i * 4 + 2) * 64 + lane], e = at[(i * 4 + 3) * 64 + lane];
-        if (d < A.dim) *(px_f32x4 *) (o + d) = (a + b) + (c + e);
+        if (d >= A.dim) continue;
+        const px_f32x4 x = (a + b) + (c + e);
+        *(px_f32x4 *) (o + d) = x;
+        odd |= !px_finite(x);
     }
+    if (odd && last && px_finite(l)) px_infinite(A, o, tok, head, 8 * wave + 4 * g, 32);
 }
 
 // part `part` of n things in shares of `share`
@@ -497,7 +542,10 @@ __global__ void __launch_bounds__(256) k_prefix_merge(const px_args A, int parts
     if (!on) return;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t r = r0 + mine;
-    *(px_f32x4 *) (A.out + r / A.heads * A.out_stride + r % A.heads * A.dim + d) = o * f;
+    float * to = A.out + r / A.heads * A.out_stride + r % A.heads * A.dim;
+    o *= f;
+    *(px_f32x4 *) (to + d) = o;
+    if (!px_finite(o) && px_finite(l)) px_infinite(A, to, (int) (r / A.heads), (int) (r % A.heads), d, A.dim);
     if (d == 0 && A.lse) A.lse[r] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.693147181f;
 }
 

@@ -761,3 +761,34 @@ def test_keys_of_minus_infinity(heads, kv, dim, tokens, prompt, own):
     mass = U.Dev(np.zeros(prompt + own, np.float32))
     p.give(mass, 0.0)
     assert np.allclose(mass.get(np.float32), w.sum((0, 1))[:prompt + own], rtol=8e-6, atol=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(32, 4, 64, 1, 200, 13), (4, 4, 128, 24, 100, 70), (8, 1, 40, 16, 129, 40), (71, 1, 72, 1, 0, 700), (24, 3, 24, 9, 1, 257), (16, 2, 80, 8, 1000, 0), (2, 1, 256, 3, 40, 0),
+                                                             (32, 32, 80, 70, 333, 0), (32, 32, 40, 70, 333, 20), (300, 300, 8, 65, 333, 0), (16, 16, 160, 128, 300, 20)])
+def test_values_of_infinity(heads, kv, dim, tokens, prompt, own):
+    """an infinite value that a token sees makes an infinity of its output, two of different signs no number; the other outputs are what they are without.  The same where the device says how many cells there are, and without a mask"""
+    U, lib = gpu()
+    rng = np.random.default_rng(dim + heads + 1)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own, loners=tokens > 1)
+    n = prompt + own
+    cells = rng.permutation(np.flatnonzero(seen.any(0)))[:5]
+    for c, value in zip(cells, (np.inf, -np.inf, np.inf, -np.inf, np.nan)):
+        v[c, rng.integers(0, kv), rng.integers(0, dim, 2)] = value
+    v[cells[0], 0, 3], v[cells[1], 0, 3] = np.inf, -np.inf               # both
+    rooms = [None, (prompt + 600, n + 900)]
+    for room in rooms + ([(n, n)] if own == 0 else []):
+        if room:
+            k, v = (np.concatenate([x, np.full((max(0, room[1] - len(x)), kv, dim), np.nan, np.float16)]) for x in (k, v))
+        with np.errstate(invalid="ignore"):
+            want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
+        fine = np.isfinite(want)
+        assert np.isinf(want).any() and fine.any()
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5, room)
+        if room == (n, n):
+            p.mask.ptr = None
+        p.attend()
+        got, lse = p.outputs()
+        for kind in (np.isposinf, np.isneginf, np.isnan):
+            assert (kind(got) == kind(want)).all(), kind
+        check_attention(np.where(fine, got, 0), np.where(fine, want, 0), lse, want_lse)
