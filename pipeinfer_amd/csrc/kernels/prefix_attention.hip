@@ -725,14 +725,15 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
         __syncthreads();
         const bool more = r + 64 < r1;
         const uint32_t sees[2][2] = { { ahead[0][0], ahead[0][1] }, { ahead[1][0], ahead[1][1] } };
+        const float of_rows[2] = { lse[cur][n], lse[cur][32 + n] };
         if (more) load(r + 64);
-        // (cells that every row sees have no test: half of the vector instructions are exponentials' then)
+        // (cells that every row sees, rows that all give something have no test: half of the vector instructions are exponentials' then)
         auto rows = [&](auto with_mask) __attribute__((always_inline)) {
 #pragma unroll
             for (int v = 0; v < 2; v++) {
                 if (r + 32 * v >= r1) continue;
                 const uint8_t * qt = lds + cur * STAGE + (32 * v + n) * KS + 16 * g;
-                const float l = lse[cur][32 * v + n];
+                const float l = of_rows[v];
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int base = mine + 32 * u;
@@ -743,6 +744,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
                             if (own && base + 32 > prompt) bits = sees[v][u];
                             if (base < prompt) bits |= base + 32 > prompt ? (1u << (prompt - base)) - 1 : ~0u;
                             if (n_kv - base < 32) bits &= (1u << (n_kv - base)) - 1;
+                            if (l == INFINITY) bits = 0;     // (a row that gives nothing, whatever its queries hold)
                         }
                         if (!__any(bits != 0)) continue;
                     }
@@ -759,7 +761,7 @@ template <int DP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_at
                 }
             }
         };
-        if (masked) rows(std::true_type{}); else rows(std::false_type{});
+        if (masked || __any((r + n < r1 && of_rows[0] == INFINITY) || (r + 32 + n < r1 && of_rows[1] == INFINITY))) rows(std::true_type{}); else rows(std::false_type{});
         if (more) store(cur ^ 1);
     }
     // a lane has 32 cells of one row of 32: through LDS, [row of 32][cell], to one cell a lane

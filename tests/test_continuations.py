@@ -792,3 +792,28 @@ def test_values_of_infinity(heads, kv, dim, tokens, prompt, own):
         for kind in (np.isposinf, np.isneginf, np.isnan):
             assert (kind(got) == kind(want)).all(), kind
         check_attention(np.where(fine, got, 0), np.where(fine, want, 0), lse, want_lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,own", [(4, 4, 64, 5, 300, 0), (8, 2, 80, 40, 700, 60), (16, 1, 128, 9, 0, 300), (71, 1, 64, 2, 65, 90)])
+def test_mass_of_rows_that_give_nothing(heads, kv, dim, tokens, prompt, own):
+    """rows of a padded batch: their lse is minus infinity, and whatever their queries hold is without effect; so is a key whose score is minus infinity"""
+    U, lib = gpu()
+    rng = np.random.default_rng(heads + dim)
+    q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, own)
+    n, scale = prompt + own, dim ** -0.5
+    q[:, :, 0] = 0.5 + rng.random((tokens, heads))
+    k[int(np.flatnonzero(seen[0])[0]), :, 0] = -np.inf
+    with np.errstate(invalid="ignore"):
+        _, want_lse, w = soft_max(q, k, v, seen, scale)
+    off = np.zeros((tokens, heads), bool)
+    off[tokens // 2] = True
+    off[-1, ::2] = True
+    want_lse[off], w[off] = -np.inf, 0.0
+    q[off] = np.array([np.nan, np.inf, -np.inf, 6e4], np.float16)[rng.integers(0, 4, off.sum())][:, None]
+    p = Pass(U, lib, q, k, v, seen, prompt, scale)
+    p.lse = U.Dev(want_lse.astype(np.float32))
+    old = rng.random(n).astype(np.float32)
+    mass = U.Dev(old)
+    p.give(mass, 0.5)
+    assert np.allclose(mass.get(np.float32), 0.5 * old.astype(np.float64) + w.sum((0, 1))[:n], rtol=8e-6, atol=1e-12)
