@@ -817,3 +817,22 @@ def test_mass_of_rows_that_give_nothing(heads, kv, dim, tokens, prompt, own):
     mass = U.Dev(old)
     p.give(mass, 0.5)
     assert np.allclose(mass.get(np.float32), 0.5 * old.astype(np.float64) + w.sum((0, 1))[:n], rtol=8e-6, atol=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [20000, 40000])
+def test_sample_between_equal_logits(vocab):
+    """equal logits, a border or u between two of them: the one that is drawn is the one by the definition or its neighbour among those that stay"""
+    U, lib = gpu()
+    x = np.zeros((4, vocab), np.float32)
+    x[1, ::3] = 1.0
+    x[2, 1::2] = -np.inf
+    x[3, :100] = 5.0
+    for u in (0.0, 0.25, 0.3, 0.5, 0.777, 1 - 2.0 ** -24):
+        for k, top_p in ((0, 1.0), (100, 1.0), (0, 0.5), (777, 0.4321), (5000, 0.75)):
+            got = run_sample(U, lib, x, vocab, (None, np.full(4, k), np.full(4, top_p), None), [u] * 4)
+            for t in range(4):
+                i, _, n, _ = sampled(x[t], np.float32(1.0), k, np.float32(top_p), np.float32(0.0), np.float32(u))
+                ids = np.flatnonzero(x[t] > -np.inf)
+                ids = np.sort(ids[np.argsort(-x[t, ids], kind="stable")][:n + 1])      # (the next one may stay, where a border is a whole count)
+                assert abs(int(got[2][t]) - n) <= 1 and got[0][t] in ids and abs(int(np.searchsorted(ids, got[0][t])) - int(np.searchsorted(ids, i))) <= 1, (t, u, k, top_p, got[0][t], i, got[2][t], n)
