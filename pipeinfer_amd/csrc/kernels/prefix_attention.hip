@@ -103,6 +103,7 @@ template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & 
         if (rises) m = top - (top - next > PX_GAP ? PX_ALONE : PX_TOP);
         else if (both <= least && top < m - PX_FALL && top > -INFINITY) m = fmaxf(top - PX_TOP, m - PX_HELD + __builtin_amdgcn_logf(sum));
         if (W.spare > 0 && !looks && __any(rises)) { W.look = W.tile + 1; W.spare--; }
+        if (looks && __any(top == -INFINITY)) W.look = W.tile + 1;        // (nothing to look at yet)
         const float f = sum == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);
         S.m = m; S.l *= f;
 #pragma unroll

@@ -836,3 +836,25 @@ def test_sample_between_equal_logits(vocab):
                 ids = np.flatnonzero(x[t] > -np.inf)
                 ids = np.sort(ids[np.argsort(-x[t, ids], kind="stable")][:n + 1])      # (the next one may stay, where a border is a whole count)
                 assert abs(int(got[2][t]) - n) <= 1 and got[0][t] in ids and abs(int(np.searchsorted(ids, got[0][t])) - int(np.searchsorted(ids, i))) <= 1, (t, u, k, top_p, got[0][t], i, got[2][t], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt,out", [(300, 300, 8, 65, 700, 300), (32, 32, 80, 70, 900, 650), (8, 2, 64, 3, 1500, 1100), (4, 1, 128, 40, 700, 500), (16, 16, 64, 1, 400, 390)])
+def test_a_run_of_keys_of_minus_infinity(heads, kv, dim, tokens, prompt, out):
+    """hundreds of cells in front whose scores are minus infinity, and low scores behind them: the first that count come late"""
+    U, lib = gpu()
+    rng = np.random.default_rng(out)
+    for low in (15.0, 40.0, 80.0):
+        q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, 0)
+        q[:, :, 0] = q[:, :, 1] = 4.0
+        k[:out, :, 0] = -np.inf
+        k[out:prompt, :, 1] = -low / 4 * dim ** 0.5
+        k, v = k[:prompt], (0.5 + rng.random((prompt, kv, dim))).astype(np.float16)
+        want, want_lse, _ = soft_max(q, k, v, seen, dim ** -0.5)
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5)
+        p.attend()
+        got, lse = p.outputs()
+        # (scores of up to 2^7 in powers of two: a sum of products is rounded once for every sixteen of them, the scale, its product with a score and the difference once each, every time by up to 2^-24 of the score: so much x ln 2 of a
+        # weight and of the lse)
+        far = ((dim + 15) // 16 + 3) * 2.0 ** -17 * np.log(2)
+        assert np.isfinite(got).all() and np.linalg.norm(got - want) <= far * np.linalg.norm(want) and np.abs(lse - want_lse).max() <= far
