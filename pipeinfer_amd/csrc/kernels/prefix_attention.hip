@@ -40,8 +40,9 @@ template <int DP> struct px_lds { static constexpr int K = 2 * DP + 16, V = (DP 
 #define PX_TOP 4.0f         /* so that the tile's largest is 2^4, which leaves room for the next tiles', */
 #define PX_ALONE 14.0f      /* or 2^14, where hardly another of the tile's is within */
 #define PX_GAP 20.0f        /*    2^20 of it */
-#define PX_LEAST 0.125f     /* it may fall when they are this or less */
-#define PX_FALL 7.0f        /* ... and the largest less than 2^-7, and rounded, at 2^-25, at 2^-18 of itself: so that it is 2^4 */
+#define PX_FEW 4.0f         /* at the first tile it falls where they are this or less, and the largest less than a half, */
+#define PX_LEAST 0.125f     /* at later ones where they are this or less */
+#define PX_FALL 7.0f        /*    and the largest less than 2^-7, and rounded, at 2^-25, at 2^-18 of itself: so that it is 2^4 */
 #define PX_HELD 60.0f       /* ... while the sums stay below 2^60: what is smaller beside them is lost to fp32 anyway */
 #define PX_ROSE 4           /* rises of a walk that are looked behind */
 #define PX_LIST 2048        /* cells of 64 words of a mask, a wave's */
@@ -89,7 +90,7 @@ template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & 
     };
     weigh();
     const bool looks = W.tile == W.look;
-    const float most = looks ? PX_FULL : PX_MOST, least = looks ? PX_LEAST : 0.0f;
+    const float most = looks ? PX_FULL : PX_MOST, least = W.tile == 0 ? PX_FEW : looks ? PX_LEAST : 0.0f;
     if (looks) W.look = 4 * W.tile + 1;
     if (__any(l > most || l <= least)) {
         float top = fmaxf(s[0], s[1]), next = fminf(s[0], s[1]);          // (next: one cell far above the others is not in it)
@@ -101,7 +102,7 @@ template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & 
         float m = S.m;
         const bool rises = both > most;
         if (rises) m = top - (top - next > PX_GAP ? PX_ALONE : PX_TOP);
-        else if (both <= least && top < m - PX_FALL && top > -INFINITY) m = fmaxf(top - PX_TOP, m - PX_HELD + __builtin_amdgcn_logf(sum));
+        else if (both <= least && top < m - (W.tile == 0 ? 1.0f : PX_FALL) && top > -INFINITY) m = fmaxf(top - PX_TOP, m - PX_HELD + __builtin_amdgcn_logf(sum));
         if (W.spare > 0 && !looks && __any(rises)) { W.look = W.tile + 1; W.spare--; }
         if (looks && __any(top == -INFINITY)) W.look = W.tile + 1;        // (nothing to look at yet)
         const float f = sum == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(S.m - m);

@@ -858,3 +858,24 @@ def test_a_run_of_keys_of_minus_infinity(heads, kv, dim, tokens, prompt, out):
         # weight and of the lse)
         far = ((dim + 15) // 16 + 3) * 2.0 ** -17 * np.log(2)
         assert np.isfinite(got).all() and np.linalg.norm(got - want) <= far * np.linalg.norm(want) and np.abs(lse - want_lse).max() <= far
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,tokens,prompt", [(300, 300, 8, 65, 700), (8, 2, 64, 3, 1500), (4, 4, 128, 1, 333), (16, 16, 64, 40, 900)])
+def test_equal_scores(heads, kv, dim, tokens, prompt):
+    """every cell the same weight, whatever the score: the mean of the values"""
+    U, lib = gpu()
+    rng = np.random.default_rng(prompt)
+    for score in (-11.0, -7.0, -5.0, -4.5, -2.0, -0.6, 0.0, 1.9, 3.3, 8.0, 30.0):
+        q, k, v, seen = inputs(rng, heads, kv, dim, tokens, prompt, 0)
+        q[:] = 0.0
+        q[:, :, 0] = 2.0
+        k, v = np.zeros((prompt, kv, dim), np.float16), (0.5 + rng.random((prompt, kv, dim))).astype(np.float16)
+        k[:, :, 0] = score / 2 * dim ** 0.5
+        p = Pass(U, lib, q, k, v, seen, prompt, dim ** -0.5)
+        p.attend()
+        got, lse = p.outputs()
+        want = np.repeat(v.astype(np.float64).mean(0), heads // kv, axis=0)[None]
+        # (The sum of the weights is rounded the same way at every one of its up to prompt / 32 additions, by 2^-24 of it at most; a weight and its two halves differ by 2^-23; the sums of the products go either way.  lse: at most 2^6, the score as in FAR)
+        far = 2.0 ** -24 * ((prompt + 31) // 32) + 2.0 ** -22
+        assert np.abs(got / want - 1).max() <= far and np.abs(lse - (2.0 * k[0, 0, 0].astype(np.float64) * dim ** -0.5 + np.log(prompt))).max() <= LSE_FAR, (score, np.abs(got / want - 1).max(), far)
