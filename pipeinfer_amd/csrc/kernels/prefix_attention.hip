@@ -637,7 +637,7 @@ extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, co
                                       int n_kv, float * scratch, size_t scratch_floats, float * out, int64_t out_stride, float * lse, const int32_t * dyn, void * stream) {
     const char * what = "pi_op_prefix_attention";
     if (px_sizes(what, head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0) return -1;
-    if (!(scale > 0.0f) || !std::isfinite(scale)) { pi_set_error("%s: scale %g (positive)", what, (double) scale); return -1; }
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.44269504f)) { pi_set_error("%s: scale %g (positive)", what, (double) scale); return -1; }
     if (n_tok == 0) return 0;
     if (!q16 || !out || (n_kv > 0 && (!k_cache || !v_cache)) || (!mask && n_kv > n_prompt)) { pi_set_error("%s: queries, caches, output or mask are NULL", what); return -1; }
     if (q_stride < (int64_t) n_head * head_dim || q_stride % 8 || out_stride < (int64_t) n_head * head_dim || out_stride % 4 || (((uintptr_t) q16 | (uintptr_t) k_cache | (uintptr_t) v_cache | (uintptr_t) out) & 15)) {
@@ -835,7 +835,7 @@ extern "C" int pi_op_attention_mass(const uint16_t * q16, int64_t q_stride, cons
                                     float decay, float * scratch, size_t scratch_floats, float * mass, const int32_t * dyn, void * stream) {
     const char * what = "pi_op_attention_mass";
     if (px_sizes(what, head_dim, n_head, n_head_kv, n_tok, n_prompt, n_kv) != 0) return -1;
-    if (!(scale > 0.0f) || !std::isfinite(scale) || !std::isfinite(decay)) { pi_set_error("%s: scale %g (positive), decay %g", what, (double) scale, (double) decay); return -1; }
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.44269504f) || !std::isfinite(decay)) { pi_set_error("%s: scale %g (positive), decay %g", what, (double) scale, (double) decay); return -1; }
     if (n_tok == 0 || n_kv == 0) return 0;
     if (!q16 || !k_cache || !lse || !mass || (!mask && n_kv > n_prompt)) { pi_set_error("%s: queries, keys, lse, mass or mask are NULL", what); return -1; }
     if (q_stride < (int64_t) n_head * head_dim || q_stride % 8 || (((uintptr_t) q16 | (uintptr_t) k_cache) & 15)) { pi_set_error("%s: rows of queries hold %d heads, %lld values apart (a multiple of 8), queries and keys on 16 bytes", what, n_head, (long long) q_stride); return -1; }

@@ -879,3 +879,11 @@ def test_equal_scores(heads, kv, dim, tokens, prompt):
         # (The sum of the weights is rounded the same way at every one of its up to prompt / 32 additions, by 2^-24 of it at most; a weight and its two halves differ by 2^-23; the sums of the products go either way.  lse: at most 2^6, the score as in FAR)
         far = 2.0 ** -24 * ((prompt + 31) // 32) + 2.0 ** -22
         assert np.abs(got / want - 1).max() <= far and np.abs(lse - (2.0 * k[0, 0, 0].astype(np.float64) * dim ** -0.5 + np.log(prompt))).max() <= LSE_FAR, (score, np.abs(got / want - 1).max(), far)
+
+
+def test_scales_that_powers_of_two_do_not_hold():
+    """scores are taken in powers of two: a scale that is infinite there is refused, not answered with no numbers"""
+    lib = L.load()
+    for scale in (2.4e38, 3.4e38):
+        assert attention_call(lib, scale=scale) != 0 and b"scale" in lib.pi_last_error()
+        assert lib.pi_op_attention_mass(P, 512, P, P, P, scale, 64, 8, 2, 3, 100, 140, 1.0, P, 1 << 40, P, None, None) != 0 and b"scale" in lib.pi_last_error()
