@@ -480,15 +480,17 @@ PI_API int pi_op_diff_attention(const float * q_dev, int64_t q_stride, const flo
 /* ---- operators of a batch of continuations of one prompt: attention over cells that all of them see, what every cell was given, a cut of the cache, a token for every row -------- */
 /* Soft-max attention over the caches of pi_op_attention (fp16 rows of n_head_kv * head_dim values per cell), all in fp32 between the products, whose tokens share their first cells:
  *   s = q . k * scale;  lse[t][h] = log sum exp(s);  out[t][h] = sum exp(s - lse) v       over the cells [0, n_prompt), which every token sees, and the cells [n_prompt, n_kv) whose bit of the token's mask is set
- * Keys and values of the prompt are read once for all tokens; a cell behind it is read for the tokens that see it, and what stands in the others is without effect (as are the mask's bits below n_prompt).  A token that sees nothing: zeros
- * and minus infinity.  q16: rows q_stride halves apart (a multiple of 8); out: rows out_stride floats apart (a multiple of 4); lse: fp32 [n_tok][n_head], nullable; mask as for pi_op_attention, nullable without such cells; heads of
- * 8 .. 256 values in steps of 8; scale positive; q16, caches, out and scratch on 16 bytes.
+ * Keys and values of the prompt serve all tokens: workgroups of 32 or 128 rows (tokens x query heads of a key head) read them, through one cache where they follow each other.  A cell behind it is read for the tokens that see it, and what
+ * stands in the others is without effect (as are the mask's bits below n_prompt).  A token that sees nothing: zeros and minus infinity.  An infinite value that a token sees makes its output infinite, two of different signs NaN.
+ * A weight is two fp16 values, together 23 bits, relative to a power of two that follows the scores: what stands beside a cell that takes nearly all keeps its bits too (behind the fifth such cell of a walk some may be held to 2^-29 of the
+ * largest only).  q16: rows q_stride halves apart (a multiple of 8); out: rows out_stride floats apart (a multiple of 4); lse: fp32 [n_tok][n_head], nullable; mask as for pi_op_attention, nullable without such cells; heads of
+ * 8 .. 256 values in steps of 8; scale positive, up to 2.35e38; q16, caches, out and scratch on 16 bytes.
  * dyn_dev (nullable): int32 {n_prompt, n_kv} in device memory, at most the arguments, which then size the split of the work and the mask's rows.  One scratch (pi_op_prefix_attention_scratch_floats; 0: none) per pass in flight */
 PI_API int pi_op_prefix_attention(const uint16_t * q16_dev, int64_t q_stride, const uint16_t * k_cache_dev, const uint16_t * v_cache_dev, const uint32_t * mask_dev, float scale, int head_dim, int n_head, int n_head_kv, int n_tok,
                                   int n_prompt, int n_kv, float * scratch_dev, size_t scratch_floats, float * out_dev, int64_t out_stride, float * lse_dev, const int32_t * dyn_dev, void * stream);
 PI_API size_t pi_op_prefix_attention_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv);
 /* What the soft-maxes of such a pass gave every cell: mass[c] <- decay * mass[c] + sum over the tokens and heads that see cell c of exp(s - lse[t][h])   (decay 0: the old mass is not read).  lse as pi_op_prefix_attention leaves it
- * (minus infinity: the row gives nothing); cells, mask, scratch and dyn_dev as there.  mass: fp32 [n_kv].  Without tokens nothing happens */
+ * (minus infinity: the row gives nothing, whatever its queries hold); cells, mask, scratch and dyn_dev as there.  mass: fp32 [n_kv].  Without tokens nothing happens */
 PI_API int pi_op_attention_mass(const uint16_t * q16_dev, int64_t q_stride, const uint16_t * k_cache_dev, const uint32_t * mask_dev, const float * lse_dev, float scale, int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt,
                                 int n_kv, float decay, float * scratch_dev, size_t scratch_floats, float * mass_dev, const int32_t * dyn_dev, void * stream);
 PI_API size_t pi_op_attention_mass_scratch_floats(int head_dim, int n_head, int n_head_kv, int n_tok, int n_prompt, int n_kv);

@@ -3,7 +3,8 @@
 //   s = q . k * scale,  p = exp(s - lse),  lse = log sum exp(s),  out = sum p v          over the cells [0, prompt) for every token, and behind them over the cells whose mask bit is set
 //   mass[cell] <- decay * mass[cell] + sum over the tokens and heads that see it of p
 //
-// The query rows of a key head - tokens x its query heads - are one matrix against the prompt's keys, so a key is read once for all of them.  The cells behind the prompt differ from token to token: a workgroup takes one
+// The query rows of a key head - tokens x its query heads - are one matrix against the prompt's keys.  A workgroup has 32 of these rows, or
+// 128, and reads the keys for them; workgroups of the same keys follow each other, on one XCD where the keys' blocks divide by 8, so that memory gives a key once and the L2 the rest.  The cells behind the prompt differ from token to token: a workgroup takes one
 // token's, listed from its mask, and reads no other, so that what stands in the others is without effect.  Scores are computed transposed (rows = cells): what a lane then holds - sixteen cells of one query - is, eight at a time, the
 // operand of the product with the values, and the values come from LDS through its transposing load.
 // Sums and statistics are fp32.  Products are fp16 x fp16 (exact in fp32); a weight is two fp16 values, rounded to nearest, the second one what the first leaves (23 bits; one alone, 11 bits, is 1.4e-4 off over 32000 cells).  fp16 ends at
@@ -659,7 +660,7 @@ extern "C" int pi_op_prefix_attention(const uint16_t * q16, int64_t q_stride, co
 
 // ---- what cells are given ---------------------------------------------------------------------------------------------------------------------------------------------------------------
 // A wave keeps the keys of 64 cells as operands and the queries of the rows go past it, 64 at a time through LDS for the four waves: a lane has 32 cells of one row of 32, adds their weights up row after row, and the lanes meet at the end.
-// Bound by the clocks of the matrix cores (27 %) and the vector unit (49 %: a factor, an exponential and a sum for every score), which hardly run at once: 64 tokens of 64 / 8 heads of 128 values, 16000 cells 43 us, 17 GFLOP.  With the cells
+// Bound by the clocks of the matrix cores (27 %) and the vector unit (49 %: a factor, an exponential and a sum for every score), which hardly run at once: 64 tokens of 64 / 8 heads of 128 values, 16000 cells 44 us, 17 GFLOP (rows that give nothing are looked for at every step: 1 us of it).  With the cells
 // on the lanes, one sum for each and a third fewer instructions, and with three waves of it on a SIMD, the time was the same, under masks 8 % longer.  8 tokens of 32 heads, 3000 cells: 10 us, the chain from the arguments to the first keys
 struct pm_args {
     const uint16_t * q; int64_t q_stride;

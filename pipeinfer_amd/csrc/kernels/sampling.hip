@@ -7,7 +7,7 @@
 //   e = exp((x - max) / temperature) of what stays (temperature 0 or less: of the first alone);  the token: in the order of the ids the first whose running sum of e exceeds u * (the sum of all), its probability e / sum
 //
 // Sums are whole numbers, weights in steps of 2^-44 (a row of 2^19 of the largest weight fits 64 bits): the order of additions, and with it of atomics, is without effect, and a sum is off by less than the number of its terms x 2^-45
-// of a total of at least 1.  Exponentials are fp64, within 1e-13: with fp32's the borders of thousands of candidates would move by whole tokens.
+// of a total of at least 1.  Exponentials are fp64, within 1.5e-13: with fp32's the borders of thousands of candidates would move by whole tokens.
 // Rows of up to 32768 logits: a workgroup each, the values in registers (k_sample).  Bound by the steps one after the other, code that runs once for the most part (1 row of 32000, top-k 40: 11 us; 64 of 32768, top-p 0.95: 39).
 //   few of the best (top_k up to 128): what every wave has its sixteenth of top_k lanes above bounds the top_k-th from below; what reaches the bound - a few times top_k values - is listed in LDS, ranked there, and one wave does the rest
 //   any number: the weights are added up in bins of equal width below the maximum, the bin that holds the border is listed and ranked
@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample_border(const sp_args A, c
     if (tid == 0) *rest = sp_rest{ best, zero, lo == 0 ? INFINITY : zero - (float) lo / unit, zero - ((float) hi + 1.5f) / unit, 1, joined, unit };
 }
 
-// Sums of a run in fp64, in an order that is always the same, then in steps; of the chances without those that are no step by themselves, so that no run of nothing but such ones is drawn.  Bound by its instructions, the fp64 ones for the most part: 22 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, so 22 us;
+// Sums of a run in fp64, in an order that is always the same, then in steps; of the chances without those that are no step by themselves, so that no run of nothing but such ones is drawn.  Bound by its instructions, the fp64 ones for the most part: 24 a value, 18 of them the two exponentials' (64 rows of 131072: with each value in steps 29, so 22 us;
 // exponentials by two and three workgroups on a compute unit 21.5, four with spilled registers 28)
 template <bool WIDE> __global__ void __launch_bounds__(512) k_sample_exact(const sp_args A, const sp_scratch S, int slices, const int32_t * __restrict__ abort_w) {
     const int gone = pi_abort_peek(abort_w), row = blockIdx.x / slices, slice = blockIdx.x % slices;
