@@ -71,7 +71,7 @@ static __device__ __forceinline__ void px_no_weights(px_weights & P) { for (int 
 // Of a tile's scores the weights and their sum; c = scale * log2(e).  S holds the products of the tiles before.
 // What weights are relative to is not the largest score: any power of two is as good that keeps them within fp16, the sums are fp32.  It rises when a lane's weights no longer fit.  A cell far above the others would leave those only fp16's
 // last bits, and where its values are small they are what the outputs are made of: so it falls again where a tile's weights are small.  That is looked for at tiles 0, 1, 5, 21, .. and behind the first rises, not at every tile: scores that
-// are far apart from tile to tile would have it follow them up and down.  (One cell of 20 above 32000 others, its values zero: 7e-7 off; relative to the largest score, both halves cut off, 1.4e-3)
+// are far apart from tile to tile would have it follow them up and down.  (One cell of 20 above 32000 others, its values zero: 7e-7 off; relative to the largest score, both halves cut off, 2.3e-4)
 template <int DP> static __device__ __forceinline__ void px_weigh(px_sums<DP> & S, px_looks & W, px_weights & P, const px_f32x16 & s, float c) {
     float p[16], l = 0.0f, minus = -1.0f;
     asm("" : "+v"(minus));                                   // (unknown to the compiler: a - h would be a conversion and a subtraction, fma takes the fp16 as it is)
@@ -417,6 +417,7 @@ static __host__ __device__ __forceinline__ int px_share_of(int n, int run, int p
 // Many rows and cells are bound by the matrix cores and the vector unit in turns (64 tokens of 64 / 8 heads of 128 values, 32000 cells: 120 us, 101 GFLOP with the weights' second halves, 840 TFLOP/s; of the clocks 45 % matrix, 40 % vector:
 // the registers of two waves are full, so little of one runs under the other); keys of their own for every head by the caches' rows (24 tokens, 2047 cells, 51 MB: 15 us, 3.4 TB/s); what lies between by the chain of a workgroup's few tiles
 // (16 tokens of 64 / 8 heads, 4000 cells, 22 MB: 15 us - 3 until the first rows are there, 5 for four runs of 32 cells a wave, 2 to meet; a token of 32 / 4 heads of 64 values, 513 cells: 8 us)
+// (Registers for four, three, two workgroups a compute unit are asked for: heads of 64 values otherwise take 170 and two fit, 100 tokens of 64 heads of 64 values, 4000 cells 36 us instead of 32)
 template <int DP, bool WIDE> __global__ void __launch_bounds__(256, DP <= 32 ? 4 : DP <= 64 ? 3 : DP <= 128 ? 2 : 1) k_prefix_attention(const px_args A, const int32_t * __restrict__ abort_w) {
     if (pi_aborted(abort_w, 5)) return;                      // (what a wave takes from LDS as an index, it has put there itself)
     constexpr int NARROW = 4 * (32 * px_lds<DP>::V + 2 * PX_LIST), MEET = 4 * DP * 128 + 1024, WIDE_B = WIDE ? 4 * 32 * (px_lds<DP>::K + px_lds<DP>::V) : MEET;
