@@ -163,7 +163,8 @@ struct px_args {
 };
 
 // Outputs that are no finite numbers although the sum of the weights `l` is: a value that the token sees is infinite, and one of a weight's two halves was zero.  They are the sum of what is not finite among its values.
-// o: the token's outputs of the head; from `d` on, every step-th four.  (Off the way: a thread reads the values of all cells, eight at a time)
+// o: the token's outputs of the head; from `d` on, every step-th four.  (Off the way: a thread reads the values of all cells, eight at a time - 1 token of 64 / 8
+// heads of 128 values over 32000 cells, one of them infinite: 5.6 ms, 64 such tokens 17)
 static __device__ __forceinline__ bool px_finite(float x) { return fabsf(x) < INFINITY; }
 static __device__ __forceinline__ bool px_finite(px_f32x4 x) { return px_finite(x[0]) && px_finite(x[1]) && px_finite(x[2]) && px_finite(x[3]); }
 static __device__ __forceinline__ void px_infinite(const px_args & A, float * o, int tok, int head, int d, int step) {
